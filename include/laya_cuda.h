@@ -234,6 +234,125 @@ int laya_matrix_apply_static(uint32_t kind, const uint8_t* w, int rows, int cols
  * ended without its budget running out. */
 int laya_wait_selftest(int device, long long budget_cycles);
 
+/* ---- operators on device buffers the caller owns ----
+ * One step of a batch of sequences over 64-token K/V pages: plan the pages
+ * of the new tokens, append their K and V, attend, read log probabilities.
+ * No counterpart in the reference (it has no K/V cache).  They take DEVICE
+ * pointers, allocate nothing, keep nothing between calls, run on `stream` (a
+ * cudaStream_t of the current device, NULL for the legacy default stream)
+ * and return without waiting for it; they may be captured into a CUDA graph
+ * (after one call on the device, which loads the module).  Arguments that
+ * the host can see are checked before any CUDA call (LAYA_E_INVALID).  What
+ * only the device sees (page numbers, slots, lengths, token ids) is checked
+ * by the kernels, which skip what is out of range and set a bit of the
+ * device's status word (laya_device_status).  Buffers that a call writes
+ * must not overlap each other or what it reads. */
+#define LAYA_TYPE_F32 0u
+#define LAYA_TYPE_F16 1u
+#define LAYA_TYPE_BF16 30u
+#define LAYA_PAGE_TOKENS 64
+
+#define LAYA_STATUS_TIMEOUT 1u /* a device-side wait ran out of its budget */
+#define LAYA_STATUS_PAGE 2u    /* a page number or slot outside the cache, or a length beyond its block table */
+#define LAYA_STATUS_TOKEN 4u   /* a token id outside the vocabulary (other than -1) */
+#define LAYA_STATUS_ROWS 8u    /* a sequence with more query rows than max_q, or offsets that are not ascending */
+
+/* Waits for the device and returns the status bits set there since the last
+ * call (ORed over all streams), clearing them. */
+int laya_device_status(int device, uint32_t* bits);
+
+/* Page plan: block tables, slot map, positions and row offsets of a step, in
+ * one launch, from the sequences' lengths.  Sequence i holds past[i] tokens in
+ * the pages of tables[i * table_stride ..] (width entries) and gets count[i]
+ * more; negative values count as 0.  Pages a sequence needs beyond
+ * ceil(past / 64) are taken from free_pages in sequence order and written to
+ * its table row (other entries are left as they were; -1 once the free list
+ * is used up, nothing past `width`).  Token rows are numbered through the
+ * sequences in order; for row t of sequence i at place u = past[i] + (t -
+ * offsets[i]):
+ *   slots[t] = tables[i][u / 64] * 64 + u % 64, or -1 without a page,
+ *   positions[t] = base + u, seqs[t] = i.
+ * Rows from the last sequence's end to `capacity`: slot -1, position 0, seq
+ * -1.  offsets[n + 1]: the sequences' first rows (cut at capacity);
+ * lens[i] = past + count; totals[2] = {token rows, pages taken}, uncut, so a
+ * caller sees totals[0] > capacity or totals[1] > n_free.  n <= 8192;
+ * positions and seqs may be NULL. */
+#define LAYA_PLAN_MAX_SEQS 8192
+int laya_page_plan(const int32_t* past, const int32_t* count, int n, const int32_t* free_pages, int n_free, int base,
+                   int32_t* tables, int64_t table_stride, int width, int64_t* slots, int32_t* positions,
+                   int32_t* seqs, int capacity, int32_t* offsets, int32_t* lens, int64_t* totals, void* stream);
+
+/* One layer's paged K and V: element (page, head, row, d) at
+ * page * page_stride + head * head_stride + row * row_stride + d (strides in
+ * elements, multiples of 8; bases 16-byte aligned), so both [pages][kv_heads]
+ * [64][head_dim] (the engine's layout) and [pages][64][kv_heads][head_dim]
+ * are described.  type LAYA_TYPE_F16 or _BF16; head_dim 64, 128 or 256. */
+typedef struct laya_kv_pages {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride;
+  int32_t pages, kv_heads, head_dim;
+  uint32_t type;
+} laya_kv_pages;
+
+/* Writes row t's kv_heads * head_dim K and V values (row strides k_stride /
+ * v_stride elements, rows 16-byte aligned) to slot slots[t] = page * 64 + row
+ * of the cache; rows with slot -1 are skipped.  `type` is the rows' type: the
+ * cache's own, or LAYA_TYPE_F32, rounded once to the nearest.  Two rows must
+ * not have the same slot (either row's 16-byte pieces may end there). */
+int laya_kv_append(const laya_kv_pages* cache, uint32_t type, const void* k, const void* v, int64_t k_stride,
+                   int64_t v_stride, const int64_t* slots, int rows, void* stream);
+
+/* Attention of a batch whose sequences share a prefix, read once for all.
+ * Query row offsets[b] + j (j < n_b = offsets[b+1] - offsets[b]) of sequence
+ * b sees the prefix (prefix_len keys in the pages prefix_pages[]) and keys 0 ..
+ * lens[b] - n_b + j of its own (lens[b] keys in the pages tables[b *
+ * table_stride ..], width entries; its new rows are the last n_b of them).
+ * o = softmax(scale q.k) v, query head h reading kv head h / (heads /
+ * kv_heads); rows that see no key give 0 and lse -inf.  Rows of no sequence
+ * are left as they were.  Scores, softmax statistics and sums are 32-bit;
+ * probabilities are rounded to the cache's type for the second product.
+ * Keys of a page outside the cache count as unseen.  Values that no row may
+ * see (past a length) may be anything, NaN included; what a sequence holds
+ * within its length has to be finite. */
+typedef struct laya_prefix_args {
+  const void* q;                /* rows x heads x head_dim, the cache's type, row stride q_stride elements */
+  int64_t q_stride;             /* a multiple of 8; q 16-byte aligned */
+  int32_t rows, heads;          /* heads a multiple of kv_heads, at most 128 to one */
+  const int32_t* offsets;       /* n_seqs + 1, ascending */
+  int32_t n_seqs, max_q;        /* max_q: the most query rows of a sequence (rows past it are not computed) */
+  const int32_t* prefix_pages;  /* ceil(prefix_len / 64) pages */
+  int32_t prefix_len;
+  int32_t width;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lens;          /* n_seqs */
+  float scale;                  /* > 0 */
+  void* out;                    /* as q, row stride out_stride (a multiple of 8, 16-byte aligned) */
+  int64_t out_stride;
+  float* lse;                   /* rows x heads: ln sum exp of the scaled scores; may be NULL */
+  void* workspace;              /* laya_prefix_attention_workspace bytes, 256-byte aligned, free for this call */
+  size_t workspace_bytes;       /* until it has run */
+} laya_prefix_args;
+/* Bytes for a call with these sizes on the current device (pointers are not looked at). */
+size_t laya_prefix_attention_workspace(const laya_kv_pages* cache, const laya_prefix_args* a);
+int laya_prefix_attention(const laya_kv_pages* cache, const laya_prefix_args* a, void* stream);
+
+/* Log probabilities from full-vocabulary logits (row i at i * row_stride
+ * elements, type F32, F16 or BF16), one read of each row:
+ *   logprobs[i][j] = log softmax(row i)[tokens[i * token_stride + j]]
+ *     (0 for a token id of -1, which pads a ragged list, or out of range),
+ *   entropy[i] (nats), lse[i] = ln sum exp(row i)   (both may be NULL),
+ *   the `top` (0..64) likeliest tokens, likeliest first, equal logits by
+ *   ascending id: top_ids / top_logprobs [rows][top].
+ * A logit of -inf is a token that is not there: it is no alternative (id -1,
+ * -inf where fewer than `top` are there), and a row of them alone has lse and
+ * logprobs -inf and entropy 0.  A row with NaN or +inf gives NaN, ids -1. */
+#define LAYA_MAX_TOP 64
+int laya_token_logprobs(uint32_t type, const void* logits, int64_t row_stride, int rows, int vocab,
+                        const int32_t* tokens, int64_t token_stride, int n_tokens, int top, float* logprobs,
+                        float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, void* stream);
+
 /* ---- timing of the last laya_decide_batch / laya_decode call ---- */
 typedef struct laya_timing {
   double device_ms;   /* CUDA-event time on the device stream(s), inputs already in HBM; max over devices */

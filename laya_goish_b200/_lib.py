@@ -65,6 +65,22 @@ class OtConfig(ctypes.Structure):
                [("theta", ctypes.c_float), ("eps", ctypes.c_float), ("layer_full", ctypes.c_void_p)]
 
 
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("pages", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("type", ctypes.c_uint32)]
+
+
+class PrefixArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("rows", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("offsets", ctypes.c_void_p), ("n_seqs", ctypes.c_int32),
+                ("max_q", ctypes.c_int32), ("prefix_pages", ctypes.c_void_p), ("prefix_len", ctypes.c_int32),
+                ("width", ctypes.c_int32), ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("lens", ctypes.c_void_p), ("scale", ctypes.c_float), ("out", ctypes.c_void_p),
+                ("out_stride", ctypes.c_int64), ("lse", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 class ProfileEntry(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("launches", ctypes.c_int64), ("total_ms", ctypes.c_double)]
 
@@ -110,6 +126,14 @@ def lib() -> ctypes.CDLL:
     L.laya_last_timing.argtypes = [P, ctypes.POINTER(Timing)]
     L.laya_profile_enable.argtypes = [P, I]
     L.laya_profile_read.argtypes = [P, ctypes.POINTER(ProfileEntry), I]
+    L.laya_device_status.argtypes = [I, P]
+    I64 = ctypes.c_int64
+    L.laya_page_plan.argtypes = [P, P, I, P, I, I, P, I64, I, P, P, P, I, P, P, P, P]
+    L.laya_kv_append.argtypes = [P, ctypes.c_uint32, P, P, I64, I64, P, I, P]
+    L.laya_prefix_attention_workspace.argtypes = [P, P]
+    L.laya_prefix_attention_workspace.restype = SZ
+    L.laya_prefix_attention.argtypes = [P, P, P]
+    L.laya_token_logprobs.argtypes = [ctypes.c_uint32, P, I64, I, I, P, I64, I, I, P, P, P, P, P, P]
     L.laya_openthai_open.argtypes = [ctypes.c_char_p, I, ctypes.POINTER(OtConfig), ctypes.POINTER(P)]
     L.laya_openthai_open_memory.argtypes = [P, SZ, I, ctypes.POINTER(OtConfig), ctypes.POINTER(P)]
     L.laya_openthai_forward.argtypes = [P, P, I, P, I, P]

@@ -1,0 +1,712 @@
+// Attention of a batch whose sequences share a prefix.
+//
+// A query row's keys are the prefix's and its own sequence's:
+//   o = sum_k e^(s_k) v_k / sum_k e^(s_k),   s = scale q.k.
+// The softmax over a union of key sets joins from each set's normalised
+// output o_s and l_s = log2 sum 2^(s_k log2 e):
+//   l = log2 sum_s 2^(l_s),   o = sum_s 2^(l_s - l) o_s,
+// so the prefix is one attention of all rows of the batch against one key
+// list (read once, not once per sequence), each sequence's own keys another,
+// and the partial results (F32) are joined.
+//
+// Launches: the prefix kernel writes its key splits' partials; the own-keys
+// kernel starts beside it (programmatic dependent launch), and waits for it
+// only before joining the partials into the output.  Own keys that are split
+// as well (few sequences with long ones) leave partials, too, and a third
+// kernel joins all.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "device_ops.h"
+#include "gemm.h"
+#include "launch.h"
+#include "mma.cuh"
+#include "ptx.cuh"
+
+namespace laya {
+
+namespace {
+
+constexpr long long kBudget = 400000000ll;  // SM cycles per bounded wait (~0.2 s)
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct PfxParams {
+  const void* q;
+  long long q_stride;
+  int rows, H, KV, G;
+  const int* offsets;
+  int n_seqs, max_q;
+  const int* prefix_pages;
+  int prefix_len;
+  const int* tables;
+  long long tstride;
+  int width;
+  const int* lens;
+  float scale_log2;
+  void* out;
+  long long out_stride;
+  float* lse;
+  float* part_o;  // [splits][rows][H][HD]: prefix splits, then own-key splits
+  float* part_l;  // [splits][rows][H], log2 units
+  int sp, ss;     // prefix splits (0: no prefix), own-key splits
+  int q_tiles;    // row tiles per sequence (own keys) or over all rows (prefix)
+  int pages;      // pages of the cache
+  unsigned* status;
+};
+
+template <typename E>
+struct Mma;
+template <>
+struct Mma<half> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma16816(d, a, b0, b1);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_h2(a, b); }
+};
+template <>
+struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Byte offset of 16-byte piece c of row r in a [HD / 64 blocks][R rows][128 B]
+// tile with 128-byte swizzle.
+template <int R>
+__device__ __forceinline__ int tile_off(int r, int c) {
+  return (c >> 3) * (R * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// A sequence's rows and keys, its device-side sizes checked.
+struct Seq {
+  int q0, nq, len, keys;  // first row, rows (at most max_q), own tokens, own keys that its table holds
+};
+__device__ __forceinline__ Seq seq_of(const PfxParams& p, int b) {
+  const int a = p.offsets[b], e = p.offsets[b + 1], l = p.lens[b];
+  Seq s;
+  s.q0 = min(max(a, 0), p.rows);
+  const int n = min(max(e, s.q0), p.rows) - s.q0;
+  s.nq = min(n, p.max_q);
+  s.len = max(l, 0) - (n - s.nq);  // so that row j sees keys 0 .. len - nq + j whether or not rows were cut
+  s.keys = (int)min((long long)max(l, 0), (long long)p.width * 64);
+  return s;
+}
+__device__ __forceinline__ void check_seq(const PfxParams& p, int b) {
+  const int a = p.offsets[b], e = p.offsets[b + 1], l = p.lens[b];
+  unsigned bad = 0;
+  if (a < 0 || e < a || e > p.rows || e - a > p.max_q) bad |= LAYA_STATUS_ROWS;
+  if (l < 0 || (long long)l > (long long)p.width * 64) bad |= LAYA_STATUS_PAGE;
+  if (bad) atomicOr(p.status, bad);
+}
+
+// Joins one row's own result (l0, log2 units; -inf: nothing) with its sp
+// prefix partials: the weights' common reference and 1 / sum of weights.
+struct Join {
+  float ref, inv, w0;
+};
+__device__ __forceinline__ Join join_row(const PfxParams& p, size_t th, float l0) {
+  const size_t plane = (size_t)p.rows * p.H;
+  Join j;
+  float m = l0;
+  for (int s = 0; s < p.sp; s++) m = fmaxf(m, p.part_l[s * plane + th]);
+  j.ref = m;
+  const float r = m == -INFINITY ? 0.f : m;
+  j.w0 = ex2(l0 - r);
+  float sum = j.w0;
+  for (int s = 0; s < p.sp; s++) sum += ex2(p.part_l[s * plane + th] - r);
+  j.inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  j.ref = m == -INFINITY ? -INFINITY : m - log2f(j.inv);
+  j.w0 *= j.inv;
+  return j;
+}
+
+template <int HD>
+struct Unit {
+  static constexpr int PAGE = 64 * HD * 2;  // K or V of one page
+  static constexpr int STAGE = 2 * PAGE;
+  static constexpr int S = HD == 64 ? 8 : HD == 128 ? 4 : 3;
+  // Warps that share a row tile's pages.  S is a multiple of it, so a stage is
+  // always the same warp's: a warp that waited for another's stage could meet
+  // its barrier a phase early and take the old phase for the new one.
+  static constexpr int NWS = HD == 256 ? 3 : 4;
+  static_assert(S % NWS == 0, "a stage belongs to one warp");
+  static constexpr int OFF_Q = S * STAGE;  // [HD / 64][ROWS][128 B], at most 64 rows
+  static constexpr int OFF_BAR = OFF_Q + 64 * HD * 2;
+  static constexpr int SMEM = OFF_BAR + 2 * S * 8 + S * 4 + 1024;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+  static_assert(4 * 16 * (HD + 2) * 4 <= S * STAGE, "the warps' merge fits the ring");
+};
+
+// Attention of a tile of query rows over a list of whole 64-token pages with
+// mma.sync m16n8k16, for few rows per key list, where the K/V bytes bound it.
+// A producer warp streams each page's K and V (128-byte swizzled boxes) into
+// a ring; four consumer warps compute.
+//   SPLITK: 16 rows; warp w takes pages w, w + NWS, ... with its own online
+//           softmax, and the warps' states are joined in shared memory.
+//   else  : 64 rows; warp w has rows 16 w .. 16 w + 15 and sees every page.
+// OWN: unit = (sequence, kv head, row tile, own-key split), rows flattened as
+// token * G + head of the group; otherwise (kv head, row tile, prefix split)
+// over all rows of the batch.
+template <typename E, int HD, bool SPLITK, bool OWN>
+__global__ void __launch_bounds__(160)
+    prefix_unit_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                       const PfxParams p) {
+  using C = Unit<HD>;
+  constexpr int ROWS = SPLITK ? 16 : 64;
+  extern __shared__ uint8_t pu_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pu_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = sm + C::OFF_Q;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  uint64_t* empty = full + C::S;
+  int* page_ok = reinterpret_cast<int*>(empty + C::S);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  int u = blockIdx.x;
+  const int splits = OWN ? p.ss : p.sp;
+  const int split = u % splits;
+  u /= splits;
+  const int kvh = u % p.KV;
+  u /= p.KV;
+  const int tile = u % p.q_tiles, b = u / p.q_tiles;
+
+  Seq sq;
+  if (OWN) {
+    sq = seq_of(p, b);
+    if (tid == 0 && kvh == 0 && tile == 0 && split == 0) check_seq(p, b);
+  } else {
+    sq = {0, p.rows, p.prefix_len, p.prefix_len};
+  }
+  const int f0 = tile * ROWS, n_flat = sq.nq * p.G;
+  const int nr = min(ROWS, n_flat - f0);  // rows of this tile
+  if (nr <= 0) {
+    pdl_wait();  // every CTA: this kernel ends after the one before it
+    return;
+  }
+  // keys that row f sees: OWN len - nq + token + 1 (may be < 1), else all
+  const int first_vis = OWN ? sq.len - sq.nq + f0 / p.G + 1 : p.prefix_len;
+  const int last_vis = min(sq.keys, OWN ? sq.len - sq.nq + (f0 + nr - 1) / p.G + 1 : p.prefix_len);
+  const int n_pages = max(0, (last_vis + 63) / 64);
+  const int per = (n_pages + splits - 1) / splits;
+  const int p0 = min(n_pages, split * per), np = min(n_pages, p0 + per) - p0;
+  const int* list = OWN ? p.tables + (long long)b * p.tstride : p.prefix_pages;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::S; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], SPLITK ? 1 : 4);
+    }
+    mbar_fence_init();
+  }
+  // Q rows as [HD / 64][ROWS][128 B], swizzled; rows past the tile are zero
+  for (int i = tid; i < ROWS * (HD / 8); i += 160) {
+    const int r = i / (HD / 8), c = i % (HD / 8);
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (r < nr) {
+      const int f = f0 + r;
+      x = *reinterpret_cast<const uint4*>(static_cast<const E*>(p.q) + (long long)(sq.q0 + f / p.G) * p.q_stride +
+                                          (kvh * p.G + f % p.G) * HD + c * 8);
+    }
+    *reinterpret_cast<uint4*>(sQ + tile_off<ROWS>(r, c)) = x;
+  }
+  __syncthreads();
+  if (!OWN) pdl_trigger();
+
+  const int g = lane >> 2, t = lane & 3;
+  const int wr = SPLITK ? 0 : warp * 16;  // this warp's first row
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float acc[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < np; i++) {
+        const int st = i % C::S;
+        if (!mbar_wait(&empty[st], ((i / C::S) & 1) ^ 1, kBudget)) {
+          atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+          break;
+        }
+        const int page = list[p0 + i];
+        const bool in = page >= 0 && page < p.pages;
+        page_ok[st] = in;
+        if (in) {
+          uint8_t* dst = sm + st * C::STAGE;
+          mbar_expect_tx(&full[st], C::STAGE);
+#pragma unroll
+          for (int hb = 0; hb < HD / 64; hb++) {
+            tma_load_4d(dst + hb * 8192, &tk, &full[st], hb * 64, 0, kvh, page);
+            tma_load_4d(dst + C::PAGE + hb * 8192, &tv, &full[st], hb * 64, 0, kvh, page);
+          }
+        } else {
+          atomicOr(p.status, LAYA_STATUS_PAGE);
+          mbar_arrive(&full[st]);
+        }
+      }
+      // no copy is in flight when the ring is reused or the CTA ends
+      for (int x = max(0, i - C::S); x < i; x++)
+        if (!mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget)) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+    }
+  } else {
+    // visible keys of this thread's two rows
+    int vis[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
+    for (int i = SPLITK ? (warp < C::NWS ? warp : np) : 0; i < np; i += SPLITK ? C::NWS : 1) {
+      const int st = i % C::S;
+      if (!mbar_wait(&full[st], (i / C::S) & 1, kBudget)) {
+        if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+        break;
+      }
+      const uint8_t* sK = sm + st * C::STAGE;
+      uint8_t* sV = sm + st * C::STAGE + C::PAGE;
+      const int key0 = (p0 + i) * 64;
+      if (page_ok[st]) {
+        if (key0 + 64 > sq.keys) {
+          // Rows past the last key may hold anything, and 0 * NaN is NaN: zero them.
+          const int from = sq.keys - key0;
+          for (int x = (SPLITK ? lane : tid); x < (64 - from) * (HD / 8); x += SPLITK ? 32 : 128)
+            *reinterpret_cast<uint4*>(sV + tile_off<64>(from + x / (HD / 8), x % (HD / 8))) =
+                make_uint4(0u, 0u, 0u, 0u);
+          if (SPLITK)
+            __syncwarp();
+          else
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+        float sc[8][4];
+#pragma unroll
+        for (int j = 0; j < 8; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+        const int mat = lane / 8;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+          uint32_t qa[4];
+          ldsm_x4(qa, sQ + tile_off<ROWS>(wr + (lane % 8) + (mat % 2) * 8, kk * 2 + mat / 2));
+#pragma unroll
+          for (int nj = 0; nj < 8; nj += 2) {
+            uint32_t bf[4];
+            ldsm_x4(bf, sK + tile_off<64>(nj * 8 + (lane % 8) + (mat / 2) * 8, kk * 2 + (mat % 2)));
+            Mma<E>::run(sc[nj], qa, bf[0], bf[1]);
+            Mma<E>::run(sc[nj + 1], qa, bf[2], bf[3]);
+          }
+        }
+        if (key0 + 64 > min(first_vis, sq.keys)) {
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (key0 + j * 8 + 2 * t + (e & 1) >= vis[e >> 1]) sc[j][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m[h], mx);
+          // a row that has seen no key yet keeps reference 0: its terms are 2^-inf = 0
+          const float ref = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2((m[h] - ref) * p.scale_log2), off = -ref * p.scale_log2;
+          m[h] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            sc[j][2 * h] = ex2(fmaf(sc[j][2 * h], p.scale_log2, off));
+            sc[j][2 * h + 1] = ex2(fmaf(sc[j][2 * h + 1], p.scale_log2, off));
+            sum += sc[j][2 * h] + sc[j][2 * h + 1];
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          l[h] = l[h] * corr + sum;
+#pragma unroll
+          for (int d = 0; d < HD / 8; d++) {
+            acc[d][2 * h] *= corr;
+            acc[d][2 * h + 1] *= corr;
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+          // probabilities rounded to the cache's type: the second product's operand
+          const uint32_t pa[4] = {Mma<E>::pack(sc[2 * kk][0], sc[2 * kk][1]), Mma<E>::pack(sc[2 * kk][2], sc[2 * kk][3]),
+                                  Mma<E>::pack(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
+                                  Mma<E>::pack(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
+#pragma unroll
+          for (int nd = 0; nd < HD / 8; nd += 2) {
+            uint32_t bf[4];
+            ldsm_x4_t(bf, sV + tile_off<64>(kk * 16 + (lane % 8) + (mat % 2) * 8, nd + mat / 2));
+            Mma<E>::run(acc[nd], pa, bf[0], bf[1]);
+            Mma<E>::run(acc[nd + 1], pa, bf[2], bf[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+  }
+  // ---- the tile's results
+  const bool partial = !OWN || p.ss > 1;
+  const int plane = OWN ? p.sp + split : split;
+  const size_t rowsH = (size_t)p.rows * p.H;
+  if (SPLITK) {
+    // join the four warps through the (drained) ring: [4][16][HD + 2]
+    __syncthreads();
+    float* comb = reinterpret_cast<float*>(sm);
+    if (warp < 4) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float* cw = comb + (warp * 16 + g + 8 * h) * (HD + 2);
+        if (t == 0) {
+          cw[0] = m[h] * p.scale_log2;
+          cw[1] = l[h];
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 8; d++) {
+          cw[2 + d * 8 + 2 * t] = acc[d][2 * h];
+          cw[2 + d * 8 + 2 * t + 1] = acc[d][2 * h + 1];
+        }
+      }
+    }
+    if (OWN) pdl_wait();  // the prefix partials
+    __syncthreads();
+    __shared__ float wts[16][8];  // the warps' weights (normalised), l or the join's weight
+    if (tid < nr) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; w++) M = fmaxf(M, comb[(w * 16 + tid) * (HD + 2)]);
+      const float r = M == -INFINITY ? 0.f : M;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        wts[tid][w] = ex2(comb[(w * 16 + tid) * (HD + 2)] - r);
+        sum += wts[tid][w] * comb[(w * 16 + tid) * (HD + 2) + 1];
+      }
+      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      const float l0 = M == -INFINITY ? -INFINITY : M - log2f(inv);
+#pragma unroll
+      for (int w = 0; w < 4; w++) wts[tid][w] *= inv;
+      const int f = f0 + tid, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
+      const size_t th = (size_t)tok * p.H + h;
+      if (partial) {
+        p.part_l[plane * rowsH + th] = l0;
+      } else {
+        const Join j = join_row(p, th, l0);
+        wts[tid][4] = j.w0;
+        wts[tid][5] = j.inv;
+        wts[tid][6] = j.ref;
+        if (p.lse) p.lse[th] = j.ref * kLn2;
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < nr * (HD / 2); i += 160) {
+      const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+      const int f = f0 + r, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
+      const size_t th = (size_t)tok * p.H + h;
+      float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float* cw = comb + (w * 16 + r) * (HD + 2) + 2 + d;
+        v0 = fmaf(wts[r][w], cw[0], v0);
+        v1 = fmaf(wts[r][w], cw[1], v1);
+      }
+      if (partial) {
+        *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d) = make_float2(v0, v1);
+      } else {
+        v0 *= wts[r][4];
+        v1 *= wts[r][4];
+        const float ref = wts[r][6];
+        for (int s = 0; s < p.sp; s++) {
+          const float ls = p.part_l[s * rowsH + th];
+          if (ls == -INFINITY) continue;
+          const float w = ex2(ls - ref);
+          const float2 o = *reinterpret_cast<const float2*>(p.part_o + (s * rowsH + th) * HD + d);
+          v0 = fmaf(w, o.x, v0);
+          v1 = fmaf(w, o.y, v1);
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + d) =
+            Mma<E>::pack(v0, v1);
+      }
+    }
+  } else {
+    if (OWN) pdl_wait();
+    if (warp < 4) {
+#pragma unroll
+      for (int hh = 0; hh < 2; hh++) {
+        const int r = wr + g + 8 * hh;
+        if (r >= nr) continue;
+        const int f = f0 + r, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
+        const size_t th = (size_t)tok * p.H + h;
+        const float inv = l[hh] > 0.f || l[hh] != l[hh] ? 1.f / l[hh] : 0.f;
+        const float l0 = m[hh] == -INFINITY ? -INFINITY : m[hh] * p.scale_log2 - log2f(inv);
+        if (partial) {
+          if (t == 0) p.part_l[plane * rowsH + th] = l0;
+#pragma unroll
+          for (int d = 0; d < HD / 8; d++)
+            *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d * 8 + 2 * t) =
+                make_float2(acc[d][2 * hh] * inv, acc[d][2 * hh + 1] * inv);
+          continue;
+        }
+        const Join j = join_row(p, th, l0);
+        if (p.lse && t == 0) p.lse[th] = j.ref * kLn2;
+        const float w0 = j.w0 * inv;
+#pragma unroll
+        for (int d = 0; d < HD / 8; d++) {
+          acc[d][2 * hh] *= w0;
+          acc[d][2 * hh + 1] *= w0;
+        }
+        for (int s = 0; s < p.sp; s++) {
+          const float ls = p.part_l[s * rowsH + th];
+          if (ls == -INFINITY) continue;
+          const float w = ex2(ls - j.ref);
+          const float* src = p.part_o + (s * rowsH + th) * HD + 2 * t;
+#pragma unroll
+          for (int d = 0; d < HD / 8; d++) {
+            const float2 o = *reinterpret_cast<const float2*>(src + d * 8);
+            acc[d][2 * hh] = fmaf(w, o.x, acc[d][2 * hh]);
+            acc[d][2 * hh + 1] = fmaf(w, o.y, acc[d][2 * hh + 1]);
+          }
+        }
+        E* dst = static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + 2 * t;
+#pragma unroll
+        for (int d = 0; d < HD / 8; d++)
+          *reinterpret_cast<uint32_t*>(dst + d * 8) = Mma<E>::pack(acc[d][2 * hh], acc[d][2 * hh + 1]);
+      }
+    }
+  }
+  // (this CTA's prefix results are visible to the dependent kernel when the
+  // whole grid has completed, which its griddepcontrol.wait waits for)
+}
+
+// Joins all partials of a row (one warp per row and head): prefix splits and
+// own-key splits.
+template <typename E, int HD>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x % 32;
+  const long long total = (long long)p.n_seqs * p.max_q * p.H, warps = (long long)gridDim.x * 8;
+  const size_t rowsH = (size_t)p.rows * p.H;
+  const int splits = p.sp + p.ss;
+  for (long long w = (long long)blockIdx.x * 8 + threadIdx.x / 32; w < total; w += warps) {
+    const int h = (int)(w % p.H), j = (int)(w / p.H % p.max_q), b = (int)(w / p.H / p.max_q);
+    const Seq s = seq_of(p, b);
+    if (j >= s.nq) continue;
+    const size_t th = (size_t)(s.q0 + j) * p.H + h;
+    float M = -INFINITY;
+    for (int i = lane; i < splits; i += 32) M = fmaxf(M, p.part_l[i * rowsH + th]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = M == -INFINITY ? 0.f : M;
+    float sum = 0.f;
+    float2 acc[HD / 64];
+#pragma unroll
+    for (int d = 0; d < HD / 64; d++) acc[d] = make_float2(0.f, 0.f);
+    for (int i = 0; i < splits; i++) {
+      const float li = p.part_l[i * rowsH + th];
+      if (li == -INFINITY) continue;
+      const float wt = ex2(li - ref);
+      sum += wt;
+#pragma unroll
+      for (int d = 0; d < HD / 64; d++) {
+        const float2 o = *reinterpret_cast<const float2*>(p.part_o + (i * rowsH + th) * HD + d * 64 + 2 * lane);
+        acc[d].x = fmaf(wt, o.x, acc[d].x);
+        acc[d].y = fmaf(wt, o.y, acc[d].y);
+      }
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    if (p.lse && lane == 0) p.lse[th] = M == -INFINITY ? -INFINITY : (M - log2f(inv)) * kLn2;
+#pragma unroll
+    for (int d = 0; d < HD / 64; d++)
+      *reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (long long)(s.q0 + j) * p.out_stride + h * HD + d * 64 +
+                                   2 * lane) = Mma<E>::pack(acc[d].x * inv, acc[d].y * inv);
+  }
+}
+
+// ------------------------------------------------------------ host
+
+// What a call's sizes decide: key splits and row tiles.
+struct Shape {
+  int sp, ss;
+  bool own_split, pre_split;  // 16-row tiles with the pages shared by the warps
+  int own_tiles, pre_tiles;
+};
+
+Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
+  Shape s{};
+  const int G = a.heads / c.kv_heads;
+  const long long flat = (long long)a.rows * G, own_flat = (long long)a.max_q * G;
+  s.own_split = own_flat <= 16;
+  s.pre_split = flat <= 16;
+  s.own_tiles = (int)((own_flat + (s.own_split ? 16 : 64) - 1) / (s.own_split ? 16 : 64));
+  s.pre_tiles = (int)((flat + (s.pre_split ? 16 : 64) - 1) / (s.pre_split ? 16 : 64));
+  const int pre_pages = (a.prefix_len + 63) / 64;
+  // Key splits until the CTAs fill the GPU once, at least two pages each.
+  const long long pre_units = (long long)s.pre_tiles * c.kv_heads;
+  if (pre_pages) s.sp = (int)std::max(1ll, std::min<long long>(sms / std::max(1ll, pre_units), (pre_pages + 1) / 2));
+  const long long own_units = (long long)a.n_seqs * s.own_tiles * c.kv_heads;
+  s.ss = (int)std::max(1ll, std::min<long long>(sms / std::max(1ll, own_units), (a.width + 7) / 8));
+  return s;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t workspace_of(const laya_kv_pages& c, const laya_prefix_args& a, const Shape& s) {
+  const size_t planes = s.sp + (s.ss > 1 ? s.ss : 0), rowsH = (size_t)a.rows * a.heads;
+  return align256(planes * rowsH * 4) + align256(planes * rowsH * c.head_dim * 4);
+}
+
+int check_sizes(const laya_kv_pages* c, const laya_prefix_args* a) {
+  if (int rc = check_pages(c)) return rc;
+  if (!a) return fail(LAYA_E_INVALID, "null argument");
+  if (a->rows < 0 || a->n_seqs < 0 || a->max_q < 0 || a->prefix_len < 0 || a->width < 0)
+    return fail(LAYA_E_INVALID, "negative size");
+  if (a->heads < 1 || a->heads % c->kv_heads) return fail(LAYA_E_INVALID, "heads must be a multiple of kv_heads");
+  if (a->heads / c->kv_heads > 128) return fail(LAYA_E_INVALID, "more than 128 query heads per kv head");
+  if ((long long)a->rows * a->heads > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many query rows");
+  return 0;
+}
+
+template <typename E, int HD, bool SPLITK, bool OWN>
+int launch_unit(const CUtensorMap& tk, const CUtensorMap& tv, const PfxParams& p, long long grid, int dev, bool pdl,
+                cudaStream_t st) {
+  static std::atomic<bool> configured[64];
+  if (!configured[dev & 63]) {
+    LAYA_CK(cudaFuncSetAttribute(prefix_unit_kernel<E, HD, SPLITK, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Unit<HD>::SMEM));
+    configured[dev & 63] = true;
+  }
+  if (grid > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many attention units");
+  LAYA_CK(launch_k(prefix_unit_kernel<E, HD, SPLITK, OWN>, dim3((unsigned)grid), dim3(160), (size_t)Unit<HD>::SMEM, st,
+                   pdl, tk, tv, p));
+  return 0;
+}
+
+template <typename E, int HD>
+int prefix_go(const CUtensorMap& tk, const CUtensorMap& tv, PfxParams p, const Shape& s, int dev, int sms,
+              cudaStream_t st) {
+  if (s.sp) {
+    p.q_tiles = s.pre_tiles;
+    const long long grid = (long long)s.pre_tiles * p.KV * s.sp;
+    if (int rc = s.pre_split ? launch_unit<E, HD, true, false>(tk, tv, p, grid, dev, false, st)
+                             : launch_unit<E, HD, false, false>(tk, tv, p, grid, dev, false, st))
+      return rc;
+  }
+  p.q_tiles = s.own_tiles;
+  const long long grid = (long long)p.n_seqs * s.own_tiles * p.KV * s.ss;
+  if (int rc = s.own_split ? launch_unit<E, HD, true, true>(tk, tv, p, grid, dev, s.sp > 0, st)
+                           : launch_unit<E, HD, false, true>(tk, tv, p, grid, dev, s.sp > 0, st))
+    return rc;
+  if (s.ss > 1) {
+    const long long total = (long long)p.n_seqs * p.max_q * p.H;
+    const int g = (int)std::min<long long>((total + 7) / 8, 16ll * sms);
+    LAYA_CK(launch_k(prefix_join_kernel<E, HD>, dim3(g), dim3(256), (size_t)0, st, true, p));
+  }
+  return 0;
+}
+
+bool page_map(CUtensorMap* m, const laya_kv_pages& c, const void* base) {
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, 64, (uint64_t)c.kv_heads, (uint64_t)c.pages};
+  const uint64_t strides[3] = {(uint64_t)c.row_stride * 2, (uint64_t)c.head_stride * 2, (uint64_t)c.page_stride * 2};
+  const uint32_t box[4] = {64, 64, 1, 1};
+  return encode_tiled(m, c.type == LAYA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                      4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace
+
+}  // namespace laya
+
+using namespace laya;
+
+extern "C" size_t laya_prefix_attention_workspace(const laya_kv_pages* cache, const laya_prefix_args* a) {
+  size_t n = 0;
+  guarded([&]() -> int {
+    if (int rc = check_sizes(cache, a)) return rc;
+    DeviceInfo di;
+    if (int rc = device_info(&di)) return rc;
+    n = workspace_of(*cache, *a, shape_of(*cache, *a, di.sms));
+    return 0;
+  });
+  return n;
+}
+
+extern "C" int laya_prefix_attention(const laya_kv_pages* cache, const laya_prefix_args* a, void* stream) {
+  return guarded([&]() -> int {
+    if (int rc = check_sizes(cache, a)) return rc;
+    if (!(a->scale > 0.f) || a->scale > 3e38f) return fail(LAYA_E_INVALID, "scale must be positive and finite");
+    if (a->rows == 0 || a->n_seqs == 0 || a->max_q == 0) return 0;
+    if (!cache->k || !cache->v || !a->q || !a->out || !a->offsets || !a->lens || (a->prefix_len && !a->prefix_pages) ||
+        (a->width && !a->tables))
+      return fail(LAYA_E_INVALID, "null argument");
+    if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v) |
+         reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15)
+      return fail(LAYA_E_INVALID, "q, out and the K/V pages must be 16-byte aligned");
+    const int64_t width = (int64_t)a->heads * cache->head_dim;
+    if (a->q_stride % 8 || a->out_stride % 8 || a->q_stride < 0 ||
+        (a->rows > 1 && (a->q_stride < width || a->out_stride < width)))
+      return fail(LAYA_E_INVALID, "query and output rows must not overlap and start on 16 bytes");
+    if (a->table_stride < a->width) return fail(LAYA_E_INVALID, "block table rows overlap");
+    DeviceInfo di;
+    if (int rc = device_info(&di)) return rc;
+    const Shape s = shape_of(*cache, *a, di.sms);
+    const size_t need = workspace_of(*cache, *a, s);
+    if (need && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 255)))
+      return fail(LAYA_E_INVALID, "workspace missing, misaligned or smaller than laya_prefix_attention_workspace");
+    PfxParams p{};
+    p.q = a->q;
+    p.q_stride = a->q_stride;
+    p.rows = a->rows;
+    p.H = a->heads;
+    p.KV = cache->kv_heads;
+    p.G = a->heads / cache->kv_heads;
+    p.offsets = a->offsets;
+    p.n_seqs = a->n_seqs;
+    p.max_q = a->max_q;
+    p.prefix_pages = a->prefix_pages;
+    p.prefix_len = a->prefix_len;
+    p.tables = a->tables;
+    p.tstride = a->table_stride;
+    p.width = a->width;
+    p.lens = a->lens;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.out = a->out;
+    p.out_stride = a->out_stride;
+    p.lse = a->lse;
+    p.sp = s.sp;
+    p.ss = s.ss;
+    const size_t planes = s.sp + (s.ss > 1 ? s.ss : 0);
+    p.part_l = static_cast<float*>(a->workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
+                                        align256(planes * (size_t)a->rows * a->heads * 4));
+    p.pages = cache->pages;
+    p.status = di.status;
+    CUtensorMap tk, tv;
+    if (!page_map(&tk, *cache, cache->k) || !page_map(&tv, *cache, cache->v))
+      return fail(LAYA_E_INVALID, "K/V pages that no tensor map can describe");
+    auto st = static_cast<cudaStream_t>(stream);
+    const bool f16 = cache->type == LAYA_TYPE_F16;
+#define LAYA_PFX(HD)                                                                          \
+  if (cache->head_dim == HD)                                                                  \
+    return f16 ? prefix_go<half, HD>(tk, tv, p, s, di.device, di.sms, st)                     \
+               : prefix_go<__nv_bfloat16, HD>(tk, tv, p, s, di.device, di.sms, st);
+    LAYA_PFX(64)
+    LAYA_PFX(128)
+    LAYA_PFX(256)
+#undef LAYA_PFX
+    return fail(LAYA_E_INVALID, "unsupported head_dim");
+  });
+}
