@@ -50,8 +50,11 @@ struct PfxParams {
   float* lse;
   float* part_o;  // [splits][rows][H][HD]: prefix splits, then own-key splits
   float* part_l;  // [splits][rows][H], log2 units
-  int sp, ss;     // prefix splits (0: no prefix), own-key splits
+  int sp, ss;     // most prefix splits of a row (0: no prefix), own-key splits
   int q_tiles;    // row tiles per sequence (own keys) or over all rows (prefix)
+  // tensor-core prefix kernel (chunk > 0): its units (kv head, unit_tok tokens)
+  // are `steps` key steps each, cut into runs of `chunk` steps over all units
+  int chunk, steps, unit_tok, n_units;
   int pages;      // pages of the cache
   unsigned* status;
 };
@@ -114,21 +117,29 @@ __device__ __forceinline__ void check_seq(const PfxParams& p, int b) {
   if (bad) atomicOr(p.status, bad);
 }
 
-// Joins one row's own result (l0, log2 units; -inf: nothing) with its sp
-// prefix partials: the weights' common reference and 1 / sum of weights.
+// Prefix splits of a row of token tok, kv head kvh.
+__device__ __forceinline__ int prefix_splits(const PfxParams& p, int tok, int kvh) {
+  if (!p.chunk || !p.sp) return p.sp;
+  const int n_tp = p.n_units / p.KV;
+  const long long u = kvh * n_tp + tok / p.unit_tok;
+  return (int)(((u + 1) * p.steps - 1) / p.chunk - u * p.steps / p.chunk) + 1;
+}
+
+// Joins one row's own result (l0, log2 units; -inf: nothing) with its
+// sp prefix partials: the weights' common reference and 1 / sum of weights.
 struct Join {
   float ref, inv, w0;
 };
-__device__ __forceinline__ Join join_row(const PfxParams& p, size_t th, float l0) {
+__device__ __forceinline__ Join join_row(const PfxParams& p, int sp, size_t th, float l0) {
   const size_t plane = (size_t)p.rows * p.H;
   Join j;
   float m = l0;
-  for (int s = 0; s < p.sp; s++) m = fmaxf(m, p.part_l[s * plane + th]);
+  for (int s = 0; s < sp; s++) m = fmaxf(m, p.part_l[s * plane + th]);
   j.ref = m;
   const float r = m == -INFINITY ? 0.f : m;
   j.w0 = ex2(l0 - r);
   float sum = j.w0;
-  for (int s = 0; s < p.sp; s++) sum += ex2(p.part_l[s * plane + th] - r);
+  for (int s = 0; s < sp; s++) sum += ex2(p.part_l[s * plane + th] - r);
   j.inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   j.ref = m == -INFINITY ? -INFINITY : m - log2f(j.inv);
   j.w0 *= j.inv;
@@ -405,7 +416,7 @@ __global__ void __launch_bounds__(160)
       if (partial) {
         p.part_l[plane * rowsH + th] = l0;
       } else {
-        const Join j = join_row(p, th, l0);
+        const Join j = join_row(p, prefix_splits(p, tok, kvh), th, l0);
         wts[tid][4] = j.w0;
         wts[tid][5] = j.inv;
         wts[tid][6] = j.ref;
@@ -430,7 +441,8 @@ __global__ void __launch_bounds__(160)
         v0 *= wts[r][4];
         v1 *= wts[r][4];
         const float ref = wts[r][6];
-        for (int s = 0; s < p.sp; s++) {
+        const int sp = prefix_splits(p, tok, kvh);
+        for (int s = 0; s < sp; s++) {
           const float ls = p.part_l[s * rowsH + th];
           if (ls == -INFINITY) continue;
           const float w = ex2(ls - ref);
@@ -461,7 +473,8 @@ __global__ void __launch_bounds__(160)
                 make_float2(acc[d][2 * hh] * inv, acc[d][2 * hh + 1] * inv);
           continue;
         }
-        const Join j = join_row(p, th, l0);
+        const int sp = prefix_splits(p, tok, kvh);
+        const Join j = join_row(p, sp, th, l0);
         if (p.lse && t == 0) p.lse[th] = j.ref * kLn2;
         const float w0 = j.w0 * inv;
 #pragma unroll
@@ -469,7 +482,7 @@ __global__ void __launch_bounds__(160)
           acc[d][2 * hh] *= w0;
           acc[d][2 * hh + 1] *= w0;
         }
-        for (int s = 0; s < p.sp; s++) {
+        for (int s = 0; s < sp; s++) {
           const float ls = p.part_l[s * rowsH + th];
           if (ls == -INFINITY) continue;
           const float w = ex2(ls - j.ref);
@@ -492,6 +505,369 @@ __global__ void __launch_bounds__(160)
   // whole grid has completed, which its griddepcontrol.wait waits for)
 }
 
+// ------------------------------------------------------------ prefix, many rows
+//
+// For more than 16 rows per kv head the prefix is a product of matrices and
+// runs on the tcgen05 tensor cores.  A unit is one kv head and NT tiles of
+// 128 query rows (a tile: TT = 128 / G tokens, row = token * G + head of the
+// group); its keys go by in steps of 128 (two pages):
+//   S = Q K^T   (M 128, N 128 into TMEM),  P = 2^(S - ref),  O += P V
+// with P written back over S in TMEM as the next product's A operand.
+//   warp 0        TMA: Q, then K and V of each step into one ring of stages
+//   warp 1        one thread issues the products; while one tile's softmax
+//                 runs, the other tile's products do
+//   warps 4 ..    softmax, four warps per tile, thread = row = TMEM lane.  O is
+//                 rescaled in TMEM only when a row's maximum passes its
+//                 reference by 2^15 (P stays below 2^15; ref = max - 7 keeps
+//                 small probabilities out of F16's subnormals).
+// Two tiles per unit halve the K/V bytes from L2 per row and keep both the
+// tensor cores (1024 cycles per tile and step at head_dim 128) and the
+// exponentials (16384 at 16 per cycle: 1024 cycles) busy; head_dim 256 has
+// room for one tile in TMEM.
+// The steps of all units, one unit after the other, are cut into equal runs,
+// one per CTA, so the GPU is evenly loaded whatever the sizes; a unit cut by a
+// run's end leaves one partial result per run (prefix_splits).
+// The last page's rows past the prefix come as zeros from a tensor map that
+// ends there, so nothing stale meets a probability of 0; pages outside the
+// cache, and a step's missing second page, are loaded out of bounds (zeros).
+template <int HD>
+struct Ptc {
+  static constexpr int NT = HD == 256 ? 1 : 2;
+  static constexpr int Q_TILE = 128 * HD * 2;  // [HD / 64][128 rows][128 B]
+  static constexpr int STAGE = 128 * HD * 2;   // K or V of a step, the same layout
+  static constexpr int NS = HD == 64 ? 10 : HD == 128 ? 5 : 2;
+  static constexpr int OFF_RING = NT * Q_TILE;
+  static constexpr int OFF_BAR = OFF_RING + NS * STAGE;
+  static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 4 * NT) * 8 + 16 + 1024;
+  static constexpr int THREADS = 128 + NT * 128;
+  // NT = 2: 168 registers per thread at launch; the first warpgroup's surplus
+  // goes to the softmax threads, which hold a row of 128 scores.
+  static constexpr int REG_LOW = 88, REG_HIGH = 208;
+  static_assert(REG_LOW + 2 * REG_HIGH <= 3 * 168, "register split");
+  static constexpr int COLS = 512;
+  static constexpr int S_COL = 0, O_COL = NT * 128;  // tile t: S at 128 t, O at O_COL + HD t
+  static_assert(O_COL + NT * HD <= COLS, "TMEM columns");
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+
+struct Run {  // a CTA's part of a unit
+  int kvh, tok0, s0, s1, plane, tiles;
+};
+
+// Part i = 0, 1, ... of CTA c's run [c * chunk, (c + 1) * chunk) of key steps.
+__device__ __forceinline__ bool run_part(const PfxParams& p, long long& at, long long end, int nt, int tt, Run& r) {
+  if (at >= end) return false;
+  const long long u = at / p.steps;
+  const int n_tp = p.n_units / p.KV;
+  r.kvh = (int)(u / n_tp);
+  r.tok0 = (int)(u % n_tp) * p.unit_tok;
+  r.s0 = (int)(at - u * p.steps);
+  r.s1 = (int)min((long long)p.steps, r.s0 + (end - at));
+  r.plane = (int)(at / p.chunk - u * p.steps / p.chunk);
+  r.tiles = min(nt, (p.rows - r.tok0 + tt - 1) / tt);
+  at += r.s1 - r.s0;
+  return true;
+}
+
+template <typename E, int HD>
+__global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tv_last,
+                     const PfxParams p) {
+  using C = Ptc<HD>;
+  constexpr int NT = C::NT;
+  extern __shared__ uint8_t pt_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = sm + C::OFF_RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);  // [NS]
+  uint64_t* empty = full + C::NS;                                 // [NS]
+  uint64_t* q_full = empty + C::NS;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;   // [NT] scores of a step
+  uint64_t* p_full = s_full + NT;   // [NT] probabilities of a step (4 warps)
+  uint64_t* o_full = p_full + NT;   // [NT] O of a part complete
+  uint64_t* o_empty = o_full + NT;  // [NT] O read (4 warps)
+  uint64_t* fin = o_empty + NT;     // all products of the CTA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int G = p.G, TT = 128 / G;
+  // tile rows that no token has (G not a divisor of 128) are zero: finite scores, never written out
+  for (int i = threadIdx.x; i < NT * (HD / 64) * (128 - TT * G) * 8; i += C::THREADS) {
+    const int per = (128 - TT * G) * 8, blk = i / per, e = i % per;
+    reinterpret_cast<uint4*>(sm + blk * 16384 + TT * G * 128)[e] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_async_smem();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::NS; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(fin, 1);
+    for (int t = 0; t < NT; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_empty[t], 4);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tbase = *tmem_slot;
+  long long at = (long long)blockIdx.x * p.chunk;
+  const long long end = min(at + p.chunk, (long long)p.n_units * p.steps);
+  const int n_pages = (p.prefix_len + 63) / 64;
+  unsigned bad = 0;
+  bool live = true;  // false once a wait ran out: every role then leaves its loops
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    if (live && !mbar_wait(b, parity, kBudget)) live = false;
+    return live;
+  };
+  Run r;
+
+  if (warp < 4) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_LOW));
+    if (warp == 0) {
+      if (lane == 0) {
+        int g = 0, k = 0;  // stages, parts
+        while (live && run_part(p, at, end, NT, TT, r)) {
+          if (!wait(q_empty, (k & 1) ^ 1)) break;
+          mbar_expect_tx(q_full, (uint32_t)(r.tiles * TT * G * 128 * (HD / 64)));
+          for (int t = 0; t < r.tiles; t++)
+#pragma unroll
+            for (int hb = 0; hb < HD / 64; hb++)
+              tma_load_3d(sm + t * C::Q_TILE + hb * 16384, &tq, q_full, hb * 64, r.kvh * G, r.tok0 + t * TT);
+          k++;
+          for (int s = r.s0; s < r.s1 && live; s++) {
+            int page[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              page[h] = 2 * s + h < n_pages ? p.prefix_pages[2 * s + h] : p.pages;
+              if (page[h] < 0 || page[h] >= p.pages) {
+                if (2 * s + h < n_pages) bad |= LAYA_STATUS_PAGE;
+                page[h] = p.pages;  // out of bounds: zeros
+              }
+            }
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+              const int st = g % C::NS;
+              if (!wait(&empty[st], ((g / C::NS) & 1) ^ 1)) break;
+              g++;
+              mbar_expect_tx(&full[st], C::STAGE);
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                const void* map = kv == 0 ? &tk : 2 * s + h == n_pages - 1 ? &tv_last : &tv;
+#pragma unroll
+                for (int hb = 0; hb < HD / 64; hb++)
+                  tma_load_4d(ring + st * C::STAGE + hb * 16384 + h * 8192, map, &full[st], hb * 64, 0, r.kvh, page[h]);
+              }
+            }
+          }
+        }
+        // the last use of every stage is over, or after a timeout its copy has
+        // landed, before the CTA may end
+        for (int x = max(0, g - C::NS); x < g; x++)
+          if (!wait(&empty[x % C::NS], (x / C::NS) & 1)) mbar_wait(&full[x % C::NS], (x / C::NS) & 1, kBudget);
+        if (!live && k) mbar_wait(q_full, (k - 1) & 1, kBudget);
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        constexpr bool BF = sizeof(E) == 2 && !__is_same(E, half);
+        const uint32_t id_s = BF ? idesc_bf16_f32(128, 128) : idesc_f16_f32(128, 128);
+        const uint32_t id_o = (BF ? idesc_bf16_f32(128, HD) : idesc_f16_f32(128, HD)) | (1u << 16);  // V MN-major
+        int g = 0, k = 0;
+        int steps_t[NT] = {}, parts_t[NT] = {};
+        while (live && run_part(p, at, end, NT, TT, r)) {
+          if (!wait(q_full, k & 1)) break;
+          k++;
+          const int ns = r.s1 - r.s0;
+          // scores of step j (ring stage g + 2 j) for tile t
+          auto scores = [&](int j, int t) {
+            const int x = g + 2 * j, st = x % C::NS;
+            if (!wait(&full[st], (x / C::NS) & 1)) return;
+            tc_fence_after();
+            const uint8_t* q = sm + t * C::Q_TILE;
+            const uint8_t* kk0 = ring + st * C::STAGE;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++)
+              umma_f16(tbase + C::S_COL + t * 128, sw128_desc(smem_u32(q + (kk >> 2) * 16384 + (kk & 3) * 32)),
+                       sw128_desc(smem_u32(kk0 + (kk >> 2) * 16384 + (kk & 3) * 32)), id_s, kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[t]);
+            if (t == r.tiles - 1) {
+              umma_commit(&empty[st]);
+              if (j == ns - 1) umma_commit(q_empty);
+            }
+          };
+          for (int t = 0; t < r.tiles; t++) scores(0, t);
+          for (int j = 0; j < ns && live; j++) {
+            const int x = g + 2 * j + 1, st = x % C::NS;
+            for (int t = 0; t < r.tiles; t++) {
+              if (j == 0) wait(&o_empty[t], (parts_t[t] & 1) ^ 1);
+              wait(&full[st], (x / C::NS) & 1);
+              if (!wait(&p_full[t], steps_t[t] & 1)) break;
+              steps_t[t]++;
+              tc_fence_after();
+              const uint8_t* v = ring + st * C::STAGE;
+#pragma unroll
+              for (int kk = 0; kk < 8; kk++)
+                umma_f16_ta(tbase + C::O_COL + t * HD, tbase + C::S_COL + t * 128 + kk * 8,
+                            sw128_mn_desc(smem_u32(v + kk * 2048), 16384, 1024), id_o, (j > 0 || kk > 0) ? 1u : 0u);
+              if (t == r.tiles - 1) umma_commit(&empty[st]);
+              if (j == ns - 1) {
+                umma_commit(&o_full[t]);
+                parts_t[t]++;
+              } else {
+                // over this tile's P: products run in the order of issue
+                scores(j + 1, t);
+              }
+            }
+          }
+          g += 2 * ns;
+        }
+        // every product is over before TMEM is freed
+        umma_commit(fin);
+        mbar_wait(fin, 0, kBudget);
+      }
+    }  // warps 2 and 3 only lend their registers
+  } else {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_HIGH));
+    const int t = (warp - 4) / 4, quarter = warp % 4, row = quarter * 32 + lane;
+    const uint32_t tl = tbase + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t tS = tl + C::S_COL + t * 128, tO = tl + C::O_COL + t * HD;
+    int step = 0, part = 0;
+    while (live && run_part(p, at, end, NT, TT, r)) {
+      if (t >= r.tiles) continue;
+      const int tok = r.tok0 + t * TT + row / G, h = r.kvh * G + row % G;
+      const bool valid = row < TT * G && tok < p.rows;
+      const bool busy = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers' count
+      float mref = -INFINITY, l = 0.f;
+      for (int s = r.s0; s < r.s1; s++, step++) {
+        // pages of this step that are in the cache
+        int lim = min(128, p.prefix_len - s * 128);
+        const int pg0 = __ldg(p.prefix_pages + 2 * s);
+        const int pg1 = 2 * s + 1 < n_pages ? __ldg(p.prefix_pages + 2 * s + 1) : 0;
+        const bool ok0 = pg0 >= 0 && pg0 < p.pages, ok1 = pg1 >= 0 && pg1 < p.pages;
+        live = __all_sync(0xffffffffu, wait(&s_full[t], step & 1));
+        if (!live) break;
+        tc_fence_after();
+        if (busy) {
+          uint32_t v[128];
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 4; c++) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+          tmem_ld_wait();
+          if (lim < 128 || !ok0 || !ok1) {
+#pragma unroll
+            for (int c = 0; c < 128; c++)
+              if (c >= lim || !(c < 64 ? ok0 : ok1)) v[c] = 0xff800000u;
+          }
+          float m4[4];
+#pragma unroll
+          for (int c = 0; c < 4; c++) m4[c] = __uint_as_float(v[c]);
+#pragma unroll
+          for (int c = 4; c < 128; c++) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(v[c]));
+          // the scale is positive, so the maximum commutes with it
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+          const float nref = mx > mref + 15.f ? mx - 7.f : mref;
+          if (s > r.s0 && __any_sync(0xffffffffu, nref != mref)) {
+            // this step's scores were issued after the last O += P V, so that one is complete
+            const float corr = nref != mref ? ex2(mref - nref) : 1.f;
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+              uint32_t o[32];
+              __syncwarp();
+              tmem_ld32(tO + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st32(tO + c * 32, o);
+            }
+            l *= corr;
+          }
+          mref = nref;
+          unsigned long long sc2, nm2, acc2[2];
+          const float off = mref == -INFINITY ? 0.f : -mref;  // nothing seen yet: every term is 2^-inf
+          asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(p.scale_log2));
+          asm("mov.b64 %0, {%1, %1};" : "=l"(nm2) : "f"(off));
+          asm("mov.b64 %0, {%1, %1};" : "=l"(acc2[0]) : "f"(0.f));
+          acc2[1] = acc2[0];
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+              unsigned long long x2, e2, p2;
+              asm("mov.b64 %0, {%1, %2};" : "=l"(x2) : "r"(v[64 * b + c]), "r"(v[64 * b + c + 1]));
+              asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e2) : "l"(x2), "l"(sc2), "l"(nm2));
+              float e0, e1;
+              asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(e2));
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+              asm("mov.b64 %0, {%1, %2};" : "=l"(p2) : "f"(e0), "f"(e1));
+              asm("add.rn.f32x2 %0, %1, %2;" : "=l"(acc2[(c >> 1) & 1]) : "l"(acc2[(c >> 1) & 1]), "l"(p2));
+              // rounded to the cache's type, the second product's operand
+              w[c >> 1] = Mma<E>::pack(e0, e1);
+            }
+            __syncwarp();
+            tmem_st32(tS + 32 * b, w);
+          }
+          float l4[4];
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(l4[0]), "=f"(l4[1]) : "l"(acc2[0]));
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(l4[2]), "=f"(l4[3]) : "l"(acc2[1]));
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      live = __all_sync(0xffffffffu, wait(&o_full[t], part & 1));
+      if (!live) break;
+      part++;
+      tc_fence_after();
+      if (busy) {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const size_t th = (size_t)tok * p.H + h, rowsH = (size_t)p.rows * p.H;
+        if (valid) p.part_l[r.plane * rowsH + th] = mref == -INFINITY ? -INFINITY : mref - log2f(inv);
+        float* dst = p.part_o + (r.plane * rowsH + th) * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(tO + c * 32, o);
+          tmem_ld_wait();
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(dst + c * 32 + i) =
+                  make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                              __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[t]);
+    }
+  }
+  if (!live) bad |= LAYA_STATUS_TIMEOUT;
+  if (bad) atomicOr(p.status, bad);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, C::COLS);
+  }
+}
+
 // Joins all partials of a row (one warp per row and head): prefix splits and
 // own-key splits.
 template <typename E, int HD>
@@ -500,14 +876,15 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p) {
   const int lane = threadIdx.x % 32;
   const long long total = (long long)p.n_seqs * p.max_q * p.H, warps = (long long)gridDim.x * 8;
   const size_t rowsH = (size_t)p.rows * p.H;
-  const int splits = p.sp + p.ss;
   for (long long w = (long long)blockIdx.x * 8 + threadIdx.x / 32; w < total; w += warps) {
     const int h = (int)(w % p.H), j = (int)(w / p.H % p.max_q), b = (int)(w / p.H / p.max_q);
     const Seq s = seq_of(p, b);
     if (j >= s.nq) continue;
     const size_t th = (size_t)(s.q0 + j) * p.H + h;
+    // planes 0 .. pre - 1 and sp .. sp + ss - 1
+    const int pre = p.sp ? prefix_splits(p, s.q0 + j, h / p.G) : 0, splits = pre + p.ss, gap = p.sp - pre;
     float M = -INFINITY;
-    for (int i = lane; i < splits; i += 32) M = fmaxf(M, p.part_l[i * rowsH + th]);
+    for (int i = lane; i < splits; i += 32) M = fmaxf(M, p.part_l[(i < pre ? i : i + gap) * rowsH + th]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ref = M == -INFINITY ? 0.f : M;
@@ -515,7 +892,8 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p) {
     float2 acc[HD / 64];
 #pragma unroll
     for (int d = 0; d < HD / 64; d++) acc[d] = make_float2(0.f, 0.f);
-    for (int i = 0; i < splits; i++) {
+    for (int i0 = 0; i0 < splits; i0++) {
+      const int i = i0 < pre ? i0 : i0 + gap;
       const float li = p.part_l[i * rowsH + th];
       if (li == -INFINITY) continue;
       const float wt = ex2(li - ref);
@@ -540,9 +918,11 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p) {
 
 // What a call's sizes decide: key splits and row tiles.
 struct Shape {
-  int sp, ss;
-  bool own_split, pre_split;  // 16-row tiles with the pages shared by the warps
-  int own_tiles, pre_tiles;
+  int sp, ss;      // most prefix splits of a row, own-key splits
+  bool own_split;  // own keys: 16-row tiles with the pages shared by the warps
+  int own_tiles;
+  bool tc;         // prefix on the tensor cores (else one 16-row tile per kv head)
+  int chunk, steps, unit_tok, n_units, grid;
 };
 
 Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
@@ -550,13 +930,22 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   const int G = a.heads / c.kv_heads;
   const long long flat = (long long)a.rows * G, own_flat = (long long)a.max_q * G;
   s.own_split = own_flat <= 16;
-  s.pre_split = flat <= 16;
   s.own_tiles = (int)((own_flat + (s.own_split ? 16 : 64) - 1) / (s.own_split ? 16 : 64));
-  s.pre_tiles = (int)((flat + (s.pre_split ? 16 : 64) - 1) / (s.pre_split ? 16 : 64));
   const int pre_pages = (a.prefix_len + 63) / 64;
-  // Key splits until the CTAs fill the GPU once, at least two pages each.
-  const long long pre_units = (long long)s.pre_tiles * c.kv_heads;
-  if (pre_pages) s.sp = (int)std::max(1ll, std::min<long long>(sms / std::max(1ll, pre_units), (pre_pages + 1) / 2));
+  s.tc = flat > 16;
+  if (pre_pages && !s.tc) {
+    // Key splits until the CTAs fill the GPU once, at least two pages each.
+    s.sp = (int)std::max(1ll, std::min<long long>(sms / c.kv_heads, (pre_pages + 1) / 2));
+  } else if (pre_pages) {
+    s.steps = (pre_pages + 1) / 2;
+    s.unit_tok = (c.head_dim == 256 ? 1 : 2) * (128 / G);
+    s.n_units = c.kv_heads * ((a.rows + s.unit_tok - 1) / s.unit_tok);
+    const long long work = (long long)s.n_units * s.steps;
+    s.chunk = (int)std::max(1ll, (work + sms - 1) / sms);
+    s.grid = (int)((work + s.chunk - 1) / s.chunk);
+    // a unit of `steps` touches at most this many runs of `chunk`
+    s.sp = (s.steps - 2 + s.chunk) / s.chunk + 1;
+  }
   const long long own_units = (long long)a.n_seqs * s.own_tiles * c.kv_heads;
   s.ss = (int)std::max(1ll, std::min<long long>(sms / std::max(1ll, own_units), (a.width + 7) / 8));
   return s;
@@ -596,14 +985,20 @@ int launch_unit(const CUtensorMap& tk, const CUtensorMap& tv, const PfxParams& p
 }
 
 template <typename E, int HD>
-int prefix_go(const CUtensorMap& tk, const CUtensorMap& tv, PfxParams p, const Shape& s, int dev, int sms,
+int prefix_go(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tv_last, PfxParams p, const Shape& s, int dev, int sms,
               cudaStream_t st) {
-  if (s.sp) {
-    p.q_tiles = s.pre_tiles;
-    const long long grid = (long long)s.pre_tiles * p.KV * s.sp;
-    if (int rc = s.pre_split ? launch_unit<E, HD, true, false>(tk, tv, p, grid, dev, false, st)
-                             : launch_unit<E, HD, false, false>(tk, tv, p, grid, dev, false, st))
-      return rc;
+  if (s.sp && !s.tc) {
+    p.q_tiles = 1;
+    if (int rc = launch_unit<E, HD, true, false>(tk, tv, p, (long long)p.KV * s.sp, dev, false, st)) return rc;
+  } else if (s.sp) {
+    using C = Ptc<HD>;
+    static std::atomic<bool> configured[64];
+    if (!configured[dev & 63]) {
+      LAYA_CK(cudaFuncSetAttribute(prefix_tc_kernel<E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+      configured[dev & 63] = true;
+    }
+    LAYA_CK(launch_k(prefix_tc_kernel<E, HD>, dim3(s.grid), dim3(C::THREADS), (size_t)C::SMEM, st, false, tq, tk, tv,
+                     tv_last, p));
   }
   p.q_tiles = s.own_tiles;
   const long long grid = (long long)p.n_seqs * s.own_tiles * p.KV * s.ss;
@@ -618,8 +1013,9 @@ int prefix_go(const CUtensorMap& tk, const CUtensorMap& tv, PfxParams p, const S
   return 0;
 }
 
-bool page_map(CUtensorMap* m, const laya_kv_pages& c, const void* base) {
-  const uint64_t dims[4] = {(uint64_t)c.head_dim, 64, (uint64_t)c.kv_heads, (uint64_t)c.pages};
+// `rows` of each page; those past it read as zeros.
+bool page_map(CUtensorMap* m, const laya_kv_pages& c, const void* base, int rows = 64) {
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)rows, (uint64_t)c.kv_heads, (uint64_t)c.pages};
   const uint64_t strides[3] = {(uint64_t)c.row_stride * 2, (uint64_t)c.head_stride * 2, (uint64_t)c.page_stride * 2};
   const uint32_t box[4] = {64, 64, 1, 1};
   return encode_tiled(m, c.type == LAYA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
@@ -694,15 +1090,29 @@ extern "C" int laya_prefix_attention(const laya_kv_pages* cache, const laya_pref
                                         align256(planes * (size_t)a->rows * a->heads * 4));
     p.pages = cache->pages;
     p.status = di.status;
-    CUtensorMap tk, tv;
-    if (!page_map(&tk, *cache, cache->k) || !page_map(&tv, *cache, cache->v))
-      return fail(LAYA_E_INVALID, "K/V pages that no tensor map can describe");
+    CUtensorMap tq{}, tk, tv, tv_last{};
+    bool ok = page_map(&tk, *cache, cache->k) && page_map(&tv, *cache, cache->v);
+    if (s.sp && s.tc) {
+      p.chunk = s.chunk;
+      p.steps = s.steps;
+      p.unit_tok = s.unit_tok;
+      p.n_units = s.n_units;
+      const uint64_t dims[3] = {(uint64_t)cache->head_dim, (uint64_t)a->heads, (uint64_t)a->rows};
+      const uint64_t strides[2] = {(uint64_t)cache->head_dim * 2, (uint64_t)a->q_stride * 2};
+      const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(128 / p.G)};
+      ok = ok && page_map(&tv_last, *cache, cache->v, (a->prefix_len - 1) % 64 + 1) &&
+           encode_tiled(&tq,
+                        cache->type == LAYA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        3, a->q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    if (!ok) return fail(LAYA_E_INVALID, "queries or K/V pages that no tensor map can describe");
     auto st = static_cast<cudaStream_t>(stream);
     const bool f16 = cache->type == LAYA_TYPE_F16;
 #define LAYA_PFX(HD)                                                                          \
   if (cache->head_dim == HD)                                                                  \
-    return f16 ? prefix_go<half, HD>(tk, tv, p, s, di.device, di.sms, st)                     \
-               : prefix_go<__nv_bfloat16, HD>(tk, tv, p, s, di.device, di.sms, st);
+    return f16 ? prefix_go<half, HD>(tq, tk, tv, tv_last, p, s, di.device, di.sms, st)        \
+               : prefix_go<__nv_bfloat16, HD>(tq, tk, tv, tv_last, p, s, di.device, di.sms, st);
     LAYA_PFX(64)
     LAYA_PFX(128)
     LAYA_PFX(256)
