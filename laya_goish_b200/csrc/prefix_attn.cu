@@ -9,11 +9,13 @@
 // list (read once, not once per sequence), each sequence's own keys another,
 // and the partial results (F32) are joined.
 //
-// Launches: the prefix kernel writes its key splits' partials; the own-keys
-// kernel starts beside it (programmatic dependent launch), and waits for it
-// only before joining the partials into the output.  Own keys that are split
-// as well (few sequences with long ones) leave partials, too, and a third
-// kernel joins all.
+// Launches: the prefix kernel and the own-keys kernel write partials (the
+// second starts as the first's CTAs leave their SMs, programmatic dependent
+// launch), and a third joins them; without a prefix, and with own keys that
+// are not split, the own-keys kernel writes the output itself.  (Joining in
+// the own-keys kernel, behind its pages, was slower: its few rows per CTA
+// expose the latency of every plane's load.  512 rows x 16384 keys x 32 heads
+// of 128: 280 us against 230.)
 #include <cuda.h>
 
 #include <algorithm>
@@ -125,60 +127,45 @@ __device__ __forceinline__ int prefix_splits(const PfxParams& p, int tok, int kv
   return (int)(((u + 1) * p.steps - 1) / p.chunk - u * p.steps / p.chunk) + 1;
 }
 
-// Joins one row's own result (l0, log2 units; -inf: nothing) with its
-// sp prefix partials: the weights' common reference and 1 / sum of weights.
-struct Join {
-  float ref, inv, w0;
-};
-__device__ __forceinline__ Join join_row(const PfxParams& p, int sp, size_t th, float l0) {
-  const size_t plane = (size_t)p.rows * p.H;
-  Join j;
-  float m = l0;
-  for (int s = 0; s < sp; s++) m = fmaxf(m, p.part_l[s * plane + th]);
-  j.ref = m;
-  const float r = m == -INFINITY ? 0.f : m;
-  j.w0 = ex2(l0 - r);
-  float sum = j.w0;
-  for (int s = 0; s < sp; s++) sum += ex2(p.part_l[s * plane + th] - r);
-  j.inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  j.ref = m == -INFINITY ? -INFINITY : m - log2f(j.inv);
-  j.w0 *= j.inv;
-  return j;
-}
-
-template <int HD>
+template <int HD, bool SPLITK>
 struct Unit {
+  static constexpr int ROWS = SPLITK ? 16 : 64;
   static constexpr int PAGE = 64 * HD * 2;  // K or V of one page
   static constexpr int STAGE = 2 * PAGE;
-  static constexpr int S = HD == 64 ? 8 : HD == 128 ? 4 : 3;
-  // Warps that share a row tile's pages.  S is a multiple of it, so a stage is
-  // always the same warp's: a warp that waited for another's stage could meet
-  // its barrier a phase early and take the old phase for the new one.
-  static constexpr int NWS = HD == 256 ? 3 : 4;
-  static_assert(S % NWS == 0, "a stage belongs to one warp");
-  static constexpr int OFF_Q = S * STAGE;  // [HD / 64][ROWS][128 B], at most 64 rows
-  static constexpr int OFF_BAR = OFF_Q + 64 * HD * 2;
+  static constexpr int S = HD == 64 ? 4 : HD == 128 ? 2 : 3;
+  // SPLITK: warps that share a row tile's pages.  S is a multiple of it, so a
+  // stage is always the same warp's: a warp that waited for another's stage
+  // could meet its barrier a phase early and take the old phase for the new.
+  static constexpr int NW = SPLITK ? (HD == 256 ? 3 : 2) : 4;
+  static constexpr int THREADS = 32 * (NW + 1);
+  static constexpr int CTAS = HD == 256 ? 1 : HD == 128 && !SPLITK ? 2 : 3;  // per SM
+  static constexpr int OFF_Q = S * STAGE;  // [HD / 64][ROWS][128 B]
+  static constexpr int OFF_BAR = OFF_Q + ROWS * HD * 2;
   static constexpr int SMEM = OFF_BAR + 2 * S * 8 + S * 4 + 1024;
-  static_assert(SMEM <= 232448, "shared memory per CTA");
-  static_assert(4 * 16 * (HD + 2) * 4 <= S * STAGE, "the warps' merge fits the ring");
+  static_assert(!SPLITK || S % NW == 0, "a stage belongs to one warp");
+  static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory per SM");
+  static_assert(NW * 16 * (HD + 2) * 4 <= S * STAGE, "the states' merge fits the ring");
 };
 
 // Attention of a tile of query rows over a list of whole 64-token pages with
 // mma.sync m16n8k16, for few rows per key list, where the K/V bytes bound it.
 // A producer warp streams each page's K and V (128-byte swizzled boxes) into
-// a ring; four consumer warps compute.
-//   SPLITK: 16 rows; warp w takes pages w, w + NWS, ... with its own online
+// a ring; NW consumer warps compute.
+//   SPLITK: 16 rows; warp w takes pages w, w + NW, ... with its own online
 //           softmax, and the warps' states are joined in shared memory.
 //   else  : 64 rows; warp w has rows 16 w .. 16 w + 15 and sees every page.
 // OWN: unit = (sequence, kv head, row tile, own-key split), rows flattened as
 // token * G + head of the group; otherwise (kv head, row tile, prefix split)
 // over all rows of the batch.
+// A unit is short (a few pages), so its chain of latencies (sizes, page
+// numbers, pages, partials, output) is hidden by other units: small rings,
+// two or three CTAs per SM (measured in DESIGN's table).
 template <typename E, int HD, bool SPLITK, bool OWN>
-__global__ void __launch_bounds__(160)
+__global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::CTAS)
     prefix_unit_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const PfxParams p) {
-  using C = Unit<HD>;
-  constexpr int ROWS = SPLITK ? 16 : 64;
+  using C = Unit<HD, SPLITK>;
+  constexpr int ROWS = C::ROWS;
   extern __shared__ uint8_t pu_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pu_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = sm + C::OFF_Q;
@@ -194,6 +181,10 @@ __global__ void __launch_bounds__(160)
   const int kvh = u % p.KV;
   u /= p.KV;
   const int tile = u % p.q_tiles, b = u / p.q_tiles;
+  const int* list = OWN ? p.tables + (long long)b * p.tstride : p.prefix_pages;
+  // the first page numbers, before the sizes that say how many count
+  const int list_len = OWN ? p.width : (p.prefix_len + 63) / 64;
+  int ids = warp == C::NW && splits == 1 && lane < list_len ? list[lane] : 0;
 
   Seq sq;
   if (OWN) {
@@ -214,7 +205,6 @@ __global__ void __launch_bounds__(160)
   const int n_pages = max(0, (last_vis + 63) / 64);
   const int per = (n_pages + splits - 1) / splits;
   const int p0 = min(n_pages, split * per), np = min(n_pages, p0 + per) - p0;
-  const int* list = OWN ? p.tables + (long long)b * p.tstride : p.prefix_pages;
 
   if (tid == 0) {
     for (int i = 0; i < C::S; i++) {
@@ -224,7 +214,7 @@ __global__ void __launch_bounds__(160)
     mbar_fence_init();
   }
   // Q rows as [HD / 64][ROWS][128 B], swizzled; rows past the tile are zero
-  for (int i = tid; i < ROWS * (HD / 8); i += 160) {
+  for (int i = tid; i < ROWS * (HD / 8); i += C::THREADS) {
     const int r = i / (HD / 8), c = i % (HD / 8);
     uint4 x = make_uint4(0u, 0u, 0u, 0u);
     if (r < nr) {
@@ -237,6 +227,9 @@ __global__ void __launch_bounds__(160)
   __syncthreads();
   if (!OWN) pdl_trigger();
 
+  const bool partial = !OWN || p.ss > 1 || p.sp > 0;
+  const int plane = OWN ? p.sp + split : split;
+  const size_t rowsH = (size_t)p.rows * p.H;
   const int g = lane >> 2, t = lane & 3;
   const int wr = SPLITK ? 0 : warp * 16;  // this warp's first row
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -244,16 +237,16 @@ __global__ void __launch_bounds__(160)
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 
-  if (warp == 4) {
-    if (lane == 0) {
-      int i = 0;
-      for (; i < np; i++) {
-        const int st = i % C::S;
-        if (!mbar_wait(&empty[st], ((i / C::S) & 1) ^ 1, kBudget)) {
-          atomicOr(p.status, LAYA_STATUS_TIMEOUT);
-          break;
-        }
-        const int page = list[p0 + i];
+  if (warp == C::NW) {
+    int i = 0;
+    for (; i < np; i++) {
+      if (i % 32 == 0 && (i || splits > 1)) ids = p0 + i + lane < n_pages ? list[p0 + i + lane] : 0;
+      const int page = __shfl_sync(0xffffffffu, ids, i % 32);
+      const int st = i % C::S;
+      int ok = 1;
+      if (lane == 0) ok = mbar_wait(&empty[st], ((i / C::S) & 1) ^ 1, kBudget);
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (lane == 0) {
         const bool in = page >= 0 && page < p.pages;
         page_ok[st] = in;
         if (in) {
@@ -269,19 +262,23 @@ __global__ void __launch_bounds__(160)
           mbar_arrive(&full[st]);
         }
       }
+    }
+    if (lane == 0) {
+      if (i < np) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
       // no copy is in flight when the ring is reused or the CTA ends
       for (int x = max(0, i - C::S); x < i; x++)
         if (!mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget)) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
     }
-  } else {
+    __syncwarp();
+  } else if (warp < C::NW) {
     // visible keys of this thread's two rows
     int vis[2];
 #pragma unroll
     for (int h = 0; h < 2; h++)
       vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
-    for (int i = SPLITK ? (warp < C::NWS ? warp : np) : 0; i < np; i += SPLITK ? C::NWS : 1) {
+    for (int i = SPLITK ? warp : 0; i < np; i += SPLITK ? C::NW : 1) {
       const int st = i % C::S;
-      if (!mbar_wait(&full[st], (i / C::S) & 1, kBudget)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (i / C::S) & 1, kBudget))) {
         if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
         break;
       }
@@ -371,14 +368,11 @@ __global__ void __launch_bounds__(160)
     }
   }
   // ---- the tile's results
-  const bool partial = !OWN || p.ss > 1;
-  const int plane = OWN ? p.sp + split : split;
-  const size_t rowsH = (size_t)p.rows * p.H;
-  if (SPLITK) {
-    // join the four warps through the (drained) ring: [4][16][HD + 2]
+  if constexpr (SPLITK) {
+    // join the warps' states through the (drained) ring: [NW][16][HD + 2]
     __syncthreads();
     float* comb = reinterpret_cast<float*>(sm);
-    if (warp < 4) {
+    if (warp < C::NW) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         float* cw = comb + (warp * 16 + g + 8 * h) * (HD + 2);
@@ -387,75 +381,41 @@ __global__ void __launch_bounds__(160)
           cw[1] = l[h];
         }
 #pragma unroll
-        for (int d = 0; d < HD / 8; d++) {
-          cw[2 + d * 8 + 2 * t] = acc[d][2 * h];
-          cw[2 + d * 8 + 2 * t + 1] = acc[d][2 * h + 1];
-        }
-      }
-    }
-    if (OWN) pdl_wait();  // the prefix partials
-    __syncthreads();
-    __shared__ float wts[16][8];  // the warps' weights (normalised), l or the join's weight
-    if (tid < nr) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; w++) M = fmaxf(M, comb[(w * 16 + tid) * (HD + 2)]);
-      const float r = M == -INFINITY ? 0.f : M;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        wts[tid][w] = ex2(comb[(w * 16 + tid) * (HD + 2)] - r);
-        sum += wts[tid][w] * comb[(w * 16 + tid) * (HD + 2) + 1];
-      }
-      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-      const float l0 = M == -INFINITY ? -INFINITY : M - log2f(inv);
-#pragma unroll
-      for (int w = 0; w < 4; w++) wts[tid][w] *= inv;
-      const int f = f0 + tid, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
-      const size_t th = (size_t)tok * p.H + h;
-      if (partial) {
-        p.part_l[plane * rowsH + th] = l0;
-      } else {
-        const Join j = join_row(p, prefix_splits(p, tok, kvh), th, l0);
-        wts[tid][4] = j.w0;
-        wts[tid][5] = j.inv;
-        wts[tid][6] = j.ref;
-        if (p.lse) p.lse[th] = j.ref * kLn2;
+        for (int d = 0; d < HD / 8; d++)
+          *reinterpret_cast<float2*>(cw + 2 + d * 8 + 2 * t) = make_float2(acc[d][2 * h], acc[d][2 * h + 1]);
       }
     }
     __syncthreads();
-    for (int i = tid; i < nr * (HD / 2); i += 160) {
+    for (int i = tid; i < nr * (HD / 2); i += C::THREADS) {
       const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
       const int f = f0 + r, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
       const size_t th = (size_t)tok * p.H + h;
-      float v0 = 0.f, v1 = 0.f;
+      float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const float* cw = comb + (w * 16 + r) * (HD + 2) + 2 + d;
-        v0 = fmaf(wts[r][w], cw[0], v0);
-        v1 = fmaf(wts[r][w], cw[1], v1);
+      for (int w = 0; w < C::NW; w++) M = fmaxf(M, comb[(w * 16 + r) * (HD + 2)]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float sum = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::NW; w++) {
+        const float* cw = comb + (w * 16 + r) * (HD + 2);
+        const float wt = ex2(cw[0] - ref);
+        const float2 x = *reinterpret_cast<const float2*>(cw + 2 + d);
+        sum = fmaf(wt, cw[1], sum);
+        v0 = fmaf(wt, x.x, v0);
+        v1 = fmaf(wt, x.y, v1);
       }
+      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      const float l2 = M == -INFINITY ? -INFINITY : M + log2f(sum);
       if (partial) {
-        *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d) = make_float2(v0, v1);
+        if (d == 0) p.part_l[plane * rowsH + th] = l2;
+        *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d) = make_float2(v0 * inv, v1 * inv);
       } else {
-        v0 *= wts[r][4];
-        v1 *= wts[r][4];
-        const float ref = wts[r][6];
-        const int sp = prefix_splits(p, tok, kvh);
-        for (int s = 0; s < sp; s++) {
-          const float ls = p.part_l[s * rowsH + th];
-          if (ls == -INFINITY) continue;
-          const float w = ex2(ls - ref);
-          const float2 o = *reinterpret_cast<const float2*>(p.part_o + (s * rowsH + th) * HD + d);
-          v0 = fmaf(w, o.x, v0);
-          v1 = fmaf(w, o.y, v1);
-        }
+        if (d == 0 && p.lse) p.lse[th] = l2 * kLn2;
         *reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + d) =
-            Mma<E>::pack(v0, v1);
+            Mma<E>::pack(v0 * inv, v1 * inv);
       }
     }
   } else {
-    if (OWN) pdl_wait();
     if (warp < 4) {
 #pragma unroll
       for (int hh = 0; hh < 2; hh++) {
@@ -464,45 +424,26 @@ __global__ void __launch_bounds__(160)
         const int f = f0 + r, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
         const size_t th = (size_t)tok * p.H + h;
         const float inv = l[hh] > 0.f || l[hh] != l[hh] ? 1.f / l[hh] : 0.f;
-        const float l0 = m[hh] == -INFINITY ? -INFINITY : m[hh] * p.scale_log2 - log2f(inv);
+        const float l2 = m[hh] == -INFINITY ? -INFINITY : m[hh] * p.scale_log2 + log2f(l[hh]);
         if (partial) {
-          if (t == 0) p.part_l[plane * rowsH + th] = l0;
+          if (t == 0) p.part_l[plane * rowsH + th] = l2;
 #pragma unroll
           for (int d = 0; d < HD / 8; d++)
             *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d * 8 + 2 * t) =
                 make_float2(acc[d][2 * hh] * inv, acc[d][2 * hh + 1] * inv);
-          continue;
-        }
-        const int sp = prefix_splits(p, tok, kvh);
-        const Join j = join_row(p, sp, th, l0);
-        if (p.lse && t == 0) p.lse[th] = j.ref * kLn2;
-        const float w0 = j.w0 * inv;
+        } else {
+          if (t == 0 && p.lse) p.lse[th] = l2 * kLn2;
+          E* dst = static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + 2 * t;
 #pragma unroll
-        for (int d = 0; d < HD / 8; d++) {
-          acc[d][2 * hh] *= w0;
-          acc[d][2 * hh + 1] *= w0;
+          for (int d = 0; d < HD / 8; d++)
+            *reinterpret_cast<uint32_t*>(dst + d * 8) = Mma<E>::pack(acc[d][2 * hh] * inv, acc[d][2 * hh + 1] * inv);
         }
-        for (int s = 0; s < sp; s++) {
-          const float ls = p.part_l[s * rowsH + th];
-          if (ls == -INFINITY) continue;
-          const float w = ex2(ls - j.ref);
-          const float* src = p.part_o + (s * rowsH + th) * HD + 2 * t;
-#pragma unroll
-          for (int d = 0; d < HD / 8; d++) {
-            const float2 o = *reinterpret_cast<const float2*>(src + d * 8);
-            acc[d][2 * hh] = fmaf(w, o.x, acc[d][2 * hh]);
-            acc[d][2 * hh + 1] = fmaf(w, o.y, acc[d][2 * hh + 1]);
-          }
-        }
-        E* dst = static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + 2 * t;
-#pragma unroll
-        for (int d = 0; d < HD / 8; d++)
-          *reinterpret_cast<uint32_t*>(dst + d * 8) = Mma<E>::pack(acc[d][2 * hh], acc[d][2 * hh + 1]);
       }
     }
   }
-  // (this CTA's prefix results are visible to the dependent kernel when the
-  // whole grid has completed, which its griddepcontrol.wait waits for)
+  // The join kernel's griddepcontrol.wait has to cover the prefix kernel, too:
+  // this one ends after it.
+  if (OWN) pdl_wait();
 }
 
 // ------------------------------------------------------------ prefix, many rows
@@ -868,50 +809,59 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
   }
 }
 
-// Joins all partials of a row (one warp per row and head): prefix splits and
-// own-key splits.
+// Joins all partials of a row: prefix splits and own-key splits.  HD / 8
+// lanes per row (token, head), eight values each; the loads of four planes are
+// in flight together.  CTA = (sequence, 256 / (HD / 8) of its rows).  Bound by
+// latency (sizes, l_s, partials: dependent loads) and by the partials' bytes,
+// which are in L2.
 template <typename E, int HD>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p) {
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p, int blocks_per_seq) {
+  constexpr int L = HD / 8, R = 256 / L;  // lanes per row, rows per CTA
+  const int b = blockIdx.x / blocks_per_seq, i0 = (blockIdx.x % blocks_per_seq) * R + threadIdx.x / L;
+  const int sub = threadIdx.x % L;
+  const Seq s = seq_of(p, b);
   pdl_wait();
-  const int lane = threadIdx.x % 32;
-  const long long total = (long long)p.n_seqs * p.max_q * p.H, warps = (long long)gridDim.x * 8;
-  const size_t rowsH = (size_t)p.rows * p.H;
-  for (long long w = (long long)blockIdx.x * 8 + threadIdx.x / 32; w < total; w += warps) {
-    const int h = (int)(w % p.H), j = (int)(w / p.H % p.max_q), b = (int)(w / p.H / p.max_q);
-    const Seq s = seq_of(p, b);
-    if (j >= s.nq) continue;
-    const size_t th = (size_t)(s.q0 + j) * p.H + h;
-    // planes 0 .. pre - 1 and sp .. sp + ss - 1
-    const int pre = p.sp ? prefix_splits(p, s.q0 + j, h / p.G) : 0, splits = pre + p.ss, gap = p.sp - pre;
-    float M = -INFINITY;
-    for (int i = lane; i < splits; i += 32) M = fmaxf(M, p.part_l[(i < pre ? i : i + gap) * rowsH + th]);
+  if (i0 >= s.nq * p.H) return;
+  const int h = i0 % p.H, tok = s.q0 + i0 / p.H;
+  const size_t rowsH = (size_t)p.rows * p.H, th = (size_t)tok * p.H + h;
+  // planes 0 .. pre - 1 and sp .. sp + ss - 1
+  const int pre = p.sp ? prefix_splits(p, tok, h / p.G) : 0, planes = pre + p.ss, gap = p.sp - pre;
+  const float* pl = p.part_l + th;
+  const float* po = p.part_o + th * HD + sub * 8;
+  float M = -INFINITY, sum = 0.f, acc[8];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = M == -INFINITY ? 0.f : M;
-    float sum = 0.f;
-    float2 acc[HD / 64];
+  for (int d = 0; d < 8; d++) acc[d] = 0.f;
+  for (int j = 0; j < planes; j += 4) {
+    float li[4], x[4][8];
 #pragma unroll
-    for (int d = 0; d < HD / 64; d++) acc[d] = make_float2(0.f, 0.f);
-    for (int i0 = 0; i0 < splits; i0++) {
-      const int i = i0 < pre ? i0 : i0 + gap;
-      const float li = p.part_l[i * rowsH + th];
-      if (li == -INFINITY) continue;
-      const float wt = ex2(li - ref);
+    for (int e = 0; e < 4; e++) {
+      const int i = min(j + e, planes - 1);
+      const size_t plane = (i < pre ? i : i + gap) * rowsH;
+      li[e] = j + e < planes ? pl[plane] : -INFINITY;
+      const float4 y = *reinterpret_cast<const float4*>(po + plane * HD);
+      const float4 z = *reinterpret_cast<const float4*>(po + plane * HD + 4);
+      x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
+      x[e][4] = z.x, x[e][5] = z.y, x[e][6] = z.z, x[e][7] = z.w;
+    }
+    const float mn = fmaxf(M, fmaxf(fmaxf(li[0], li[1]), fmaxf(li[2], li[3])));
+    const float ref = mn == -INFINITY ? 0.f : mn, corr = ex2(M - ref);
+    M = mn;
+    sum *= corr;
+#pragma unroll
+    for (int d = 0; d < 8; d++) acc[d] *= corr;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float wt = ex2(li[e] - ref);
       sum += wt;
 #pragma unroll
-      for (int d = 0; d < HD / 64; d++) {
-        const float2 o = *reinterpret_cast<const float2*>(p.part_o + (i * rowsH + th) * HD + d * 64 + 2 * lane);
-        acc[d].x = fmaf(wt, o.x, acc[d].x);
-        acc[d].y = fmaf(wt, o.y, acc[d].y);
-      }
+      for (int d = 0; d < 8; d++) acc[d] = fmaf(wt, x[e][d], acc[d]);
     }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    if (p.lse && lane == 0) p.lse[th] = M == -INFINITY ? -INFINITY : (M - log2f(inv)) * kLn2;
-#pragma unroll
-    for (int d = 0; d < HD / 64; d++)
-      *reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (long long)(s.q0 + j) * p.out_stride + h * HD + d * 64 +
-                                   2 * lane) = Mma<E>::pack(acc[d].x * inv, acc[d].y * inv);
   }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  if (p.lse && sub == 0) p.lse[th] = M == -INFINITY ? -INFINITY : (M + log2f(sum)) * kLn2;
+  *reinterpret_cast<uint4*>(static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + sub * 8) =
+      make_uint4(Mma<E>::pack(acc[0] * inv, acc[1] * inv), Mma<E>::pack(acc[2] * inv, acc[3] * inv),
+                 Mma<E>::pack(acc[4] * inv, acc[5] * inv), Mma<E>::pack(acc[6] * inv, acc[7] * inv));
 }
 
 // ------------------------------------------------------------ host
@@ -933,6 +883,7 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   s.own_tiles = (int)((own_flat + (s.own_split ? 16 : 64) - 1) / (s.own_split ? 16 : 64));
   const int pre_pages = (a.prefix_len + 63) / 64;
   s.tc = flat > 16;
+  static const int kMinChunk = getenv("PFX_MIN") ? atoi(getenv("PFX_MIN")) : 1;
   if (pre_pages && !s.tc) {
     // Key splits until the CTAs fill the GPU once, at least two pages each.
     s.sp = (int)std::max(1ll, std::min<long long>(sms / c.kv_heads, (pre_pages + 1) / 2));
@@ -941,7 +892,7 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
     s.unit_tok = (c.head_dim == 256 ? 1 : 2) * (128 / G);
     s.n_units = c.kv_heads * ((a.rows + s.unit_tok - 1) / s.unit_tok);
     const long long work = (long long)s.n_units * s.steps;
-    s.chunk = (int)std::max(1ll, (work + sms - 1) / sms);
+    s.chunk = (int)std::max<long long>(kMinChunk, (work + sms - 1) / sms);
     s.grid = (int)((work + s.chunk - 1) / s.chunk);
     // a unit of `steps` touches at most this many runs of `chunk`
     s.sp = (s.steps - 2 + s.chunk) / s.chunk + 1;
@@ -954,7 +905,7 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t workspace_of(const laya_kv_pages& c, const laya_prefix_args& a, const Shape& s) {
-  const size_t planes = s.sp + (s.ss > 1 ? s.ss : 0), rowsH = (size_t)a.rows * a.heads;
+  const size_t planes = s.sp || s.ss > 1 ? s.sp + s.ss : 0, rowsH = (size_t)a.rows * a.heads;
   return align256(planes * rowsH * 4) + align256(planes * rowsH * c.head_dim * 4);
 }
 
@@ -975,11 +926,11 @@ int launch_unit(const CUtensorMap& tk, const CUtensorMap& tv, const PfxParams& p
   static std::atomic<bool> configured[64];
   if (!configured[dev & 63]) {
     LAYA_CK(cudaFuncSetAttribute(prefix_unit_kernel<E, HD, SPLITK, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Unit<HD>::SMEM));
+                                 Unit<HD, SPLITK>::SMEM));
     configured[dev & 63] = true;
   }
   if (grid > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many attention units");
-  LAYA_CK(launch_k(prefix_unit_kernel<E, HD, SPLITK, OWN>, dim3((unsigned)grid), dim3(160), (size_t)Unit<HD>::SMEM, st,
+  LAYA_CK(launch_k(prefix_unit_kernel<E, HD, SPLITK, OWN>, dim3((unsigned)grid), dim3(Unit<HD, SPLITK>::THREADS), (size_t)Unit<HD, SPLITK>::SMEM, st,
                    pdl, tk, tv, p));
   return 0;
 }
@@ -1005,10 +956,12 @@ int prefix_go(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& t
   if (int rc = s.own_split ? launch_unit<E, HD, true, true>(tk, tv, p, grid, dev, s.sp > 0, st)
                            : launch_unit<E, HD, false, true>(tk, tv, p, grid, dev, s.sp > 0, st))
     return rc;
-  if (s.ss > 1) {
-    const long long total = (long long)p.n_seqs * p.max_q * p.H;
-    const int g = (int)std::min<long long>((total + 7) / 8, 16ll * sms);
-    LAYA_CK(launch_k(prefix_join_kernel<E, HD>, dim3(g), dim3(256), (size_t)0, st, true, p));
+  if (s.ss > 1 || s.sp) {
+    const int per_cta = 256 / (HD / 8);
+    const long long blocks = ((long long)std::min(p.max_q, p.rows) * p.H + per_cta - 1) / per_cta;
+    if (blocks * p.n_seqs > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many attention rows");
+    LAYA_CK(launch_k(prefix_join_kernel<E, HD>, dim3((unsigned)(blocks * p.n_seqs)), dim3(256), (size_t)0, st, true, p,
+                     (int)blocks));
   }
   return 0;
 }
@@ -1084,7 +1037,7 @@ extern "C" int laya_prefix_attention(const laya_kv_pages* cache, const laya_pref
     p.lse = a->lse;
     p.sp = s.sp;
     p.ss = s.ss;
-    const size_t planes = s.sp + (s.ss > 1 ? s.ss : 0);
+    const size_t planes = s.sp || s.ss > 1 ? s.sp + s.ss : 0;
     p.part_l = static_cast<float*>(a->workspace);
     p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
                                         align256(planes * (size_t)a->rows * a->heads * 4));

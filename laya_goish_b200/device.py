@@ -31,41 +31,55 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 STATUS_TIMEOUT, STATUS_PAGE, STATUS_TOKEN, STATUS_ROWS = 1, 2, 4, 8
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise LayaError(E_INVALID, message)
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without making a Stream object
+_current = torch._C._cuda_getDevice
+
+
+def _refuse(message: str):
+    raise LayaError(E_INVALID, message)
 
 
 def _tensor(x, name: str, dim: int, dtype=None, device=None) -> None:
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
-    _need(x.dim() == dim, f"{name} must have {dim} dimension(s)")
-    _need(dtype is None or x.dtype == dtype, f"{name} must be {dtype}")
-    _need(device is None or x.device == device, f"{name} is on another device")
-    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient; the operators are forward only")
+    # plain tests: a message is only put together when one fails (a call costs a few microseconds)
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        _refuse(f"{name} must be a CUDA tensor")
+    if x.dim() != dim:
+        _refuse(f"{name} must have {dim} dimension(s)")
+    if dtype is not None and x.dtype is not dtype:
+        _refuse(f"{name} must be {dtype}")
+    if device is not None and x.device != device:
+        _refuse(f"{name} is on another device")
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name} requires a gradient; the operators are forward only")
 
 
 def _flat(x, name: str, dtype, device) -> None:
     _tensor(x, name, 1, dtype, device)
-    _need(x.is_contiguous(), f"{name} must be contiguous")
+    if not x.is_contiguous():
+        _refuse(f"{name} must be contiguous")
 
 
 def _rows(x, name: str) -> int:
     """Row stride of a tensor whose rows (everything past dimension 0) are contiguous."""
+    shape, stride = x.shape, x.stride()
     width = 1
-    for d in range(x.dim() - 1, 0, -1):
-        _need(x.shape[d] == 1 or x.stride(d) == width, f"the rows of {name} must be contiguous")
-        width *= x.shape[d]
-    return x.stride(0) if x.shape[0] > 1 else width
+    for d in range(len(shape) - 1, 0, -1):
+        if shape[d] != 1 and stride[d] != width:
+            _refuse(f"the rows of {name} must be contiguous")
+        width *= shape[d]
+    return stride[0] if shape[0] > 1 else width
 
 
 def _call(device, fn, *args):
     """Runs a library entry point with the tensors' device current, on its current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, stream))
+    index = device.index
+    if _current() == index:
+        rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream))
+            rc = fn(*args, _stream(index))
+    if rc < 0:
+        check(rc)
 
 
 def check_status(device: int = 0) -> None:
@@ -79,7 +93,8 @@ def check_status(device: int = 0) -> None:
                             (STATUS_TOKEN, "a token id outside the vocabulary"),
                             (STATUS_ROWS, "more query rows in a sequence than max_q, or offsets out of order"))
              if bits.value & b]
-    _need(not words, "; ".join(words))
+    if words:
+        _refuse("; ".join(words))
 
 
 class PagePlan(NamedTuple):
@@ -102,20 +117,26 @@ def page_plan(past, count, free_pages, tables, capacity: int, base: int = 0) -> 
     _tensor(tables, "tables", 2, torch.int32)
     dev = tables.device
     n, width = tables.shape
-    for x, name in ((past, "past"), (count, "count"), (free_pages, "free_pages")):
-        _flat(x, name, torch.int32, dev)
-    _need(past.shape[0] == n and count.shape[0] == n, "past, count and tables must have one row per sequence")
-    _need(n == 0 or width <= 1 or tables.stride(1) == 1, "the rows of tables must be contiguous")
+    _flat(past, "past", torch.int32, dev)
+    _flat(count, "count", torch.int32, dev)
+    _flat(free_pages, "free_pages", torch.int32, dev)
+    if past.shape[0] != n or count.shape[0] != n:
+        _refuse("past, count and tables must have one row per sequence")
+    if n and width > 1 and tables.stride(1) != 1:
+        _refuse("the rows of tables must be contiguous")
     stride = tables.stride(0) if n > 1 else width
-    _need(stride >= width, "the rows of tables overlap")
-    _need(0 <= capacity < 1 << 31, "capacity out of range")
-    _need(0 <= base < 1 << 31, "base out of range")
-    slots = torch.empty(capacity, dtype=torch.int64, device=dev)
-    positions = torch.empty(capacity, dtype=torch.int32, device=dev)
-    seqs = torch.empty(capacity, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n + 1, dtype=torch.int32, device=dev)
-    lens = torch.empty(n, dtype=torch.int32, device=dev)
-    totals = torch.empty(2, dtype=torch.int64, device=dev)
+    if stride < width:
+        _refuse("the rows of tables overlap")
+    if not 0 <= capacity < 1 << 31:
+        _refuse("capacity out of range")
+    if not 0 <= base < 1 << 31:
+        _refuse("base out of range")
+    # the outputs share one allocation, each on 16 bytes
+    a, c, m = -capacity % 4, 2 * (capacity % 2), (n + 1 + 3) // 4 * 4
+    slots, _, positions, _, seqs, _, offsets, _, lens, _, totals = torch.split_with_sizes(
+        tables.new_empty(4 * capacity + c + 2 * a + 2 * m + 4),
+        (2 * capacity, c, capacity, a, capacity, a, n + 1, m - n - 1, n, m - n, 4))
+    slots, totals = slots.view(torch.int64), totals.view(torch.int64)[:2]
     _call(dev, _lib.lib().laya_page_plan, past.data_ptr(), count.data_ptr(), n, free_pages.data_ptr(),
           free_pages.shape[0], base, tables.data_ptr(), stride, width, slots.data_ptr(), positions.data_ptr(),
           seqs.data_ptr(), capacity, offsets.data_ptr(), lens.data_ptr(), totals.data_ptr())
@@ -130,22 +151,29 @@ class KVPages:
     def __init__(self, k, v):
         _tensor(k, "k pages", 4)
         _tensor(v, "v pages", 4, k.dtype, k.device)
-        _need(k.dtype in (torch.float16, torch.bfloat16), "K/V pages must be F16 or BF16")
-        _need(k.shape == v.shape, "k and v pages must have the same shape")
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            _refuse("K/V pages must be F16 or BF16")
+        if k.shape != v.shape:
+            _refuse("k and v pages must have the same shape")
         pages, heads, rows, hd = k.shape
-        _need(rows == PAGE, "a page holds 64 tokens")
-        _need(hd in (64, 128, 256), "head_dim must be 64, 128 or 256")
-        _need(pages > 0 and heads > 0, "empty K/V cache")
-        _need(k.stride(3) == 1 and v.stride(3) == 1, "head vectors must be contiguous")
+        if rows != PAGE:
+            _refuse("a page holds 64 tokens")
+        if hd not in (64, 128, 256):
+            _refuse("head_dim must be 64, 128 or 256")
+        if not pages or not heads:
+            _refuse("empty K/V cache")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            _refuse("head vectors must be contiguous")
         # strides of dimensions of one element say nothing
         stride = [k.stride(d) if k.shape[d] > 1 else hd for d in range(3)]
-        _need(all(v.stride(d) == stride[d] for d in range(3) if v.shape[d] > 1),
-              "k and v pages must have the same strides")
-        _need(all(s % 8 == 0 for s in stride) and (k.data_ptr() | v.data_ptr()) % 16 == 0,
-              "K/V pages must be 16-byte aligned")
+        if any(v.stride(d) != stride[d] for d in range(3) if v.shape[d] > 1):
+            _refuse("k and v pages must have the same strides")
+        if any(s % 8 for s in stride) or (k.data_ptr() | v.data_ptr()) % 16:
+            _refuse("K/V pages must be 16-byte aligned")
         last = 0
         for s, size in sorted((stride[d], k.shape[d]) for d in range(3)):  # each dimension past the one inside it
-            _need(size == 1 or s >= last + hd, "K/V pages overlap")
+            if size > 1 and s < last + hd:
+                _refuse("K/V pages overlap")
             last += s * (size - 1)
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.pages, self.kv_heads, self.head_dim = pages, heads, hd
@@ -158,13 +186,15 @@ def kv_append(pages: KVPages, k, v, slots) -> None:
     """Writes rows k, v ([rows, kv_heads, head_dim], the pages' type or F32, which
     is rounded once) to their slots ([rows] int64; -1: skipped; all others
     distinct)."""
-    _need(isinstance(pages, KVPages), "pages must be KVPages")
+    if not isinstance(pages, KVPages):
+        _refuse("pages must be KVPages")
     _tensor(k, "k", 3, None, pages.device)
     _tensor(v, "v", 3, k.dtype, pages.device)
     _flat(slots, "slots", torch.int64, pages.device)
-    _need(k.dtype in (pages.dtype, torch.float32), "k and v must be of the pages' type or F32")
-    _need(k.shape == v.shape and tuple(k.shape) == (slots.shape[0], pages.kv_heads, pages.head_dim),
-          "k and v must be [rows, kv_heads, head_dim] with a slot per row")
+    if k.dtype not in (pages.dtype, torch.float32):
+        _refuse("k and v must be of the pages' type or F32")
+    if k.shape != v.shape or tuple(k.shape) != (slots.shape[0], pages.kv_heads, pages.head_dim):
+        _refuse("k and v must be [rows, kv_heads, head_dim] with a slot per row")
     _call(pages.device, _lib.lib().laya_kv_append, pages._ref, TYPES[k.dtype], k.data_ptr(), v.data_ptr(),
           _rows(k, "k"), _rows(v, "v"), slots.data_ptr(), k.shape[0])
 
@@ -178,43 +208,51 @@ def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, l
     scale defaults to head_dim ** -0.5.  Returns out; rows of no sequence are
     left as they were (0 in an out made here), rows that see no key give 0.
     lse ([rows, heads] F32, optional) receives ln sum exp of the scores."""
-    _need(isinstance(pages, KVPages), "pages must be KVPages")
+    if not isinstance(pages, KVPages):
+        _refuse("pages must be KVPages")
     dev = pages.device
     _tensor(q, "q", 3, pages.dtype, dev)
     rows, heads, hd = q.shape
-    _need(hd == pages.head_dim, "q and the pages have different head_dim")
-    _need(heads > 0 and heads % pages.kv_heads == 0, "heads must be a multiple of kv_heads")
+    if hd != pages.head_dim:
+        _refuse("q and the pages have different head_dim")
+    if not heads or heads % pages.kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
     _flat(prefix_pages, "prefix_pages", torch.int32, dev)
     _flat(lens, "lens", torch.int32, dev)
     _flat(offsets, "offsets", torch.int32, dev)
     _tensor(tables, "tables", 2, torch.int32, dev)
     n, width = tables.shape
-    _need(lens.shape[0] == n and offsets.shape[0] == n + 1, "lens, offsets and tables must fit the sequences")
-    _need(n == 0 or width <= 1 or tables.stride(1) == 1, "the rows of tables must be contiguous")
-    _need(0 <= prefix_len <= prefix_pages.shape[0] * PAGE, "prefix_pages must hold prefix_len tokens")
-    _need(0 <= max_q < 1 << 31, "max_q out of range")
+    if lens.shape[0] != n or offsets.shape[0] != n + 1:
+        _refuse("lens, offsets and tables must fit the sequences")
+    if n and width > 1 and tables.stride(1) != 1:
+        _refuse("the rows of tables must be contiguous")
+    if not 0 <= prefix_len <= prefix_pages.shape[0] * PAGE:
+        _refuse("prefix_pages must hold prefix_len tokens")
+    if not 0 <= max_q < 1 << 31:
+        _refuse("max_q out of range")
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if out is None:
         out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     else:
         _tensor(out, "out", 3, pages.dtype, dev)
-        _need(out.shape == q.shape, "out must have q's shape")
+        if out.shape != q.shape:
+            _refuse("out must have q's shape")
     if lse is not None:
         _tensor(lse, "lse", 2, torch.float32, dev)
-        _need(tuple(lse.shape) == (rows, heads) and lse.is_contiguous(), "lse must be contiguous [rows, heads]")
+        if tuple(lse.shape) != (rows, heads) or not lse.is_contiguous():
+            _refuse("lse must be contiguous [rows, heads]")
+    if _current() != dev.index:  # the workspace goes by the device that runs the call
+        with torch.cuda.device(dev):
+            return prefix_attention(q, pages, prefix_pages, prefix_len, tables, lens, offsets, max_q, scale, out, lse)
     L = _lib.lib()
     a = _lib.PrefixArgs(q.data_ptr(), _rows(q, "q"), rows, heads, offsets.data_ptr(), n, max_q,
                         prefix_pages.data_ptr(), prefix_len, width, tables.data_ptr(),
                         tables.stride(0) if n > 1 else width, lens.data_ptr(), scale, out.data_ptr(),
                         _rows(out, "out"), None if lse is None else lse.data_ptr(), None, 0)
     ref = ctypes.byref(a)
-    if torch.cuda.current_device() == dev.index:
-        a.workspace_bytes = L.laya_prefix_attention_workspace(pages._ref, ref)
-    else:
-        with torch.cuda.device(dev):
-            a.workspace_bytes = L.laya_prefix_attention_workspace(pages._ref, ref)
-    if a.workspace_bytes:
-        work = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
+    a.workspace_bytes = size = L.laya_prefix_attention_workspace(pages._ref, ref)
+    if size:
+        work = q.new_empty(size, dtype=torch.uint8)
         a.workspace = work.data_ptr()
     _call(dev, L.laya_prefix_attention, pages._ref, ref)
     return out
@@ -236,18 +274,20 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     64) likeliest tokens.  Logits of -inf are tokens that are not there."""
     _tensor(logits, "logits", 2)
     dev = logits.device
-    _need(logits.dtype in TYPES, "logits must be F32, F16 or BF16")
+    if logits.dtype not in TYPES:
+        _refuse("logits must be F32, F16 or BF16")
     n, vocab = logits.shape
-    _need(vocab > 0, "empty vocabulary")
+    if not vocab:
+        _refuse("empty vocabulary")
     _tensor(tokens, "tokens", 2, torch.int32, dev)
-    _need(tokens.shape[0] == n, "tokens must have a row per row of logits")
-    _need(0 <= top <= MAX_TOP, "top must be 0..64")
+    if tokens.shape[0] != n:
+        _refuse("tokens must have a row per row of logits")
+    if not 0 <= top <= MAX_TOP:
+        _refuse("top must be 0..64")
     c = tokens.shape[1]
-    logprobs = torch.empty((n, c), dtype=torch.float32, device=dev)
-    stats = torch.empty((2, n), dtype=torch.float32, device=dev)
-    ids = torch.empty((n, top), dtype=torch.int32, device=dev)
-    top_lp = torch.empty((n, top), dtype=torch.float32, device=dev)
-    entropy, lse = stats[0], stats[1]
+    logprobs, entropy, lse, top_lp, ids = torch.split_with_sizes(
+        logits.new_empty(n * (c + 2 + 2 * top), dtype=torch.float32), (n * c, n, n, n * top, n * top))
+    logprobs, top_lp, ids = logprobs.view(n, c), top_lp.view(n, top), ids.view(torch.int32).view(n, top)
     _call(dev, _lib.lib().laya_token_logprobs, TYPES[logits.dtype], logits.data_ptr(), _rows(logits, "logits"), n,
           vocab, tokens.data_ptr(), _rows(tokens, "tokens") if c else 0, c, top, logprobs.data_ptr(),
           entropy.data_ptr(), lse.data_ptr(), ids.data_ptr(), top_lp.data_ptr())
