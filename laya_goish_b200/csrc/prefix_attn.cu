@@ -476,9 +476,10 @@ struct Ptc {
   static constexpr int NT = HD == 256 ? 1 : 2;
   static constexpr int Q_TILE = 128 * HD * 2;  // [HD / 64][128 rows][128 B]
   static constexpr int STAGE = 128 * HD * 2;   // K or V of a step, the same layout
-  static constexpr int NS = HD == 64 ? 10 : HD == 128 ? 5 : 2;
+  static constexpr int NS = HD == 64 ? 9 : HD == 128 ? 4 : 2;
   static constexpr int OFF_RING = NT * Q_TILE;
-  static constexpr int OFF_BAR = OFF_RING + NS * STAGE;
+  static constexpr int OFF_OUT = OFF_RING + NS * STAGE;  // 32 x 32 F32 per softmax warp, for coalesced partials
+  static constexpr int OFF_BAR = OFF_OUT + NT * 4 * 4096;
   static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 4 * NT) * 8 + 16 + 1024;
   static constexpr int THREADS = 128 + NT * 128;
   // NT = 2: 168 registers per thread at launch; the first warpgroup's surplus
@@ -778,19 +779,32 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const size_t th = (size_t)tok * p.H + h, rowsH = (size_t)p.rows * p.H;
         if (valid) p.part_l[r.plane * rowsH + th] = mref == -INFINITY ? -INFINITY : mref - log2f(inv);
-        float* dst = p.part_o + (r.plane * rowsH + th) * HD;
+        // a lane holds a row; through shared memory 8 lanes write 128 bytes of one
+        // (16-byte pieces, piece j of row i at j ^ (i % 8))
+        uint4* stage = reinterpret_cast<uint4*>(sm + C::OFF_OUT) + (warp - 4) * 256;
+        const int mine = valid ? (int)th : -1;
+        int rows8[8];  // the rows lane / 8, lane / 8 + 4, ... that this lane writes
+#pragma unroll
+        for (int i = 0; i < 8; i++) rows8[i] = __shfl_sync(0xffffffffu, mine, i * 4 + lane / 8);
 #pragma unroll
         for (int c = 0; c < HD / 32; c++) {
           uint32_t o[32];
           __syncwarp();
           tmem_ld32(tO + c * 32, o);
           tmem_ld_wait();
-          if (valid) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(dst + c * 32 + i) =
-                  make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
-                              __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+          for (int j = 0; j < 8; j++)
+            stage[lane * 8 + (j ^ (lane & 7))] =
+                make_uint4(__float_as_uint(__uint_as_float(o[4 * j]) * inv), __float_as_uint(__uint_as_float(o[4 * j + 1]) * inv),
+                           __float_as_uint(__uint_as_float(o[4 * j + 2]) * inv),
+                           __float_as_uint(__uint_as_float(o[4 * j + 3]) * inv));
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int row = i * 4 + lane / 8;
+            const uint4 x = stage[row * 8 + ((lane & 7) ^ (row & 7))];
+            if (rows8[i] >= 0)
+              *reinterpret_cast<uint4*>(p.part_o + (r.plane * rowsH + rows8[i]) * HD + c * 32 + (lane & 7) * 4) = x;
           }
         }
       }
