@@ -1,4 +1,5 @@
-"""Builds liblaya_cuda.so in-tree for sm_100a (nvcc cross-compiles without a GPU).
+"""Builds liblaya_cuda.so in-tree for sm_100a (nvcc cross-compiles without a GPU),
+and _device.so, the Python binding of the operators on torch tensors.
 
     python -m laya_goish_b200.build          # incremental
     python -m laya_goish_b200.build --clean  # full rebuild
@@ -11,12 +12,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(PKG, "liblaya_cuda.so")
+EXT_SRC = os.path.join(CSRC, "python", "device_ext.cpp")
+EXT_OUT = os.path.join(PKG, "_device.so")
 BUILD = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
@@ -43,18 +47,55 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _compile_ext() -> str:
+    """The binding's object file (torch's headers, the host compiler)."""
+    obj = os.path.join(BUILD, "device_ext.o")
+    newest = max(os.path.getmtime(f) for f in [EXT_SRC] + glob.glob(os.path.join(INCLUDE, "*.h")))
+    if os.path.exists(obj) and os.path.getmtime(obj) >= newest:
+        return obj
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(NVCC)) if os.path.isabs(NVCC) else "/usr/local/cuda"
+    dirs = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(cuda, "include"), *cpp_extension.include_paths()]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in dirs], "-c", EXT_SRC,
+           "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {EXT_SRC}:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link_ext(obj: str) -> None:
+    if os.path.exists(EXT_OUT) and os.path.getmtime(EXT_OUT) >= os.path.getmtime(obj):
+        return
+    from torch.utils import cpp_extension
+
+    libs = [f"-L{d}" for d in cpp_extension.library_paths()]
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", EXT_OUT + ".tmp", obj, f"-L{PKG}", "-l:liblaya_cuda.so",
+           "-Wl,-rpath,$ORIGIN", *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(EXT_OUT + ".tmp", EXT_OUT)
+
+
 def build(clean: bool = False) -> str:
     if clean and os.path.isdir(BUILD):
         shutil.rmtree(BUILD)
     os.makedirs(BUILD, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
+        ext = ex.submit(_compile_ext)
         objs = list(ex.map(_compile, _sources()))
+        ext_obj = ext.result()
     if not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", OUT + ".tmp", *objs, "-lpthread"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(OUT + ".tmp", OUT)
+    _link_ext(ext_obj)
     return OUT
 
 

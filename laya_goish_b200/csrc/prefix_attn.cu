@@ -133,16 +133,19 @@ struct Unit {
   static constexpr int PAGE = 64 * HD * 2;  // K or V of one page
   static constexpr int STAGE = 2 * PAGE;
   static constexpr int S = HD == 64 ? 4 : HD == 128 ? 2 : 3;
-  // SPLITK: warps that share a row tile's pages.  S is a multiple of it, so a
-  // stage is always the same warp's: a warp that waited for another's stage
-  // could meet its barrier a phase early and take the old phase for the new.
-  static constexpr int NW = SPLITK ? (HD == 256 ? 3 : 2) : 4;
+  // SPLITK: two warps share a page (32 keys each), PW pages are in work at a
+  // time.  S is a multiple of PW, so a stage is always the same warps': a warp
+  // that waited for another's stage could meet its barrier a phase early and
+  // take the old phase for the new.
+  static constexpr int PW = HD == 256 ? 3 : 2;
+  static constexpr int NW = SPLITK ? 2 * PW : 4;
+  static constexpr int KEYS = SPLITK ? 32 : 64;  // of a page per warp
   static constexpr int THREADS = 32 * (NW + 1);
   static constexpr int CTAS = HD == 256 ? 1 : HD == 128 && !SPLITK ? 2 : 3;  // per SM
   static constexpr int OFF_Q = S * STAGE;  // [HD / 64][ROWS][128 B]
   static constexpr int OFF_BAR = OFF_Q + ROWS * HD * 2;
   static constexpr int SMEM = OFF_BAR + 2 * S * 8 + S * 4 + 1024;
-  static_assert(!SPLITK || S % NW == 0, "a stage belongs to one warp");
+  static_assert(!SPLITK || S % PW == 0, "a stage belongs to the same warps");
   static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory per SM");
   static_assert(NW * 16 * (HD + 2) * 4 <= S * STAGE, "the states' merge fits the ring");
 };
@@ -151,8 +154,9 @@ struct Unit {
 // mma.sync m16n8k16, for few rows per key list, where the K/V bytes bound it.
 // A producer warp streams each page's K and V (128-byte swizzled boxes) into
 // a ring; NW consumer warps compute.
-//   SPLITK: 16 rows; warp w takes pages w, w + NW, ... with its own online
-//           softmax, and the warps' states are joined in shared memory.
+//   SPLITK: 16 rows; warps 2 w and 2 w + 1 take halves of pages w, w + PW, ...
+//           with online softmaxes of their own, and the warps' states are joined
+//           in shared memory.
 //   else  : 64 rows; warp w has rows 16 w .. 16 w + 15 and sees every page.
 // OWN: unit = (sequence, kv head, row tile, own-key split), rows flattened as
 // token * G + head of the group; otherwise (kv head, row tile, prefix split)
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
   if (tid == 0) {
     for (int i = 0; i < C::S; i++) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], SPLITK ? 1 : 4);
+      mbar_init(&empty[i], SPLITK ? 2 : 4);
     }
     mbar_fence_init();
   }
@@ -276,7 +280,9 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
 #pragma unroll
     for (int h = 0; h < 2; h++)
       vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
-    for (int i = SPLITK ? warp : 0; i < np; i += SPLITK ? C::NW : 1) {
+    constexpr int KEYS = C::KEYS;
+    const int koff = SPLITK ? (warp & 1) * 32 : 0;  // this warp's first key of a page
+    for (int i = SPLITK ? warp >> 1 : 0; i < np; i += SPLITK ? C::PW : 1) {
       const int st = i % C::S;
       if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (i / C::S) & 1, kBudget))) {
         if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
@@ -288,8 +294,8 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
       if (page_ok[st]) {
         if (key0 + 64 > sq.keys) {
           // Rows past the last key may hold anything, and 0 * NaN is NaN: zero them.
-          const int from = sq.keys - key0;
-          for (int x = (SPLITK ? lane : tid); x < (64 - from) * (HD / 8); x += SPLITK ? 32 : 128)
+          const int from = max(sq.keys - key0, koff);
+          for (int x = (SPLITK ? lane : tid); x < (koff + KEYS - from) * (HD / 8); x += SPLITK ? 32 : 128)
             *reinterpret_cast<uint4*>(sV + tile_off<64>(from + x / (HD / 8), x % (HD / 8))) =
                 make_uint4(0u, 0u, 0u, 0u);
           if (SPLITK)
@@ -297,34 +303,34 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
           else
             asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        float sc[8][4];
+        float sc[KEYS / 8][4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+        for (int j = 0; j < KEYS / 8; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
         const int mat = lane / 8;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; kk++) {
           uint32_t qa[4];
           ldsm_x4(qa, sQ + tile_off<ROWS>(wr + (lane % 8) + (mat % 2) * 8, kk * 2 + mat / 2));
 #pragma unroll
-          for (int nj = 0; nj < 8; nj += 2) {
+          for (int nj = 0; nj < KEYS / 8; nj += 2) {
             uint32_t bf[4];
-            ldsm_x4(bf, sK + tile_off<64>(nj * 8 + (lane % 8) + (mat / 2) * 8, kk * 2 + (mat % 2)));
+            ldsm_x4(bf, sK + tile_off<64>(koff + nj * 8 + (lane % 8) + (mat / 2) * 8, kk * 2 + (mat % 2)));
             Mma<E>::run(sc[nj], qa, bf[0], bf[1]);
             Mma<E>::run(sc[nj + 1], qa, bf[2], bf[3]);
           }
         }
         if (key0 + 64 > min(first_vis, sq.keys)) {
 #pragma unroll
-          for (int j = 0; j < 8; j++)
+          for (int j = 0; j < KEYS / 8; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              if (key0 + j * 8 + 2 * t + (e & 1) >= vis[e >> 1]) sc[j][e] = -INFINITY;
+              if (key0 + koff + j * 8 + 2 * t + (e & 1) >= vis[e >> 1]) sc[j][e] = -INFINITY;
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           float mx = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
+          for (int j = 0; j < KEYS / 8; j++) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float mn = fmaxf(m[h], mx);
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
           m[h] = mn;
           float sum = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
+          for (int j = 0; j < KEYS / 8; j++) {
             sc[j][2 * h] = ex2(fmaf(sc[j][2 * h], p.scale_log2, off));
             sc[j][2 * h + 1] = ex2(fmaf(sc[j][2 * h + 1], p.scale_log2, off));
             sum += sc[j][2 * h] + sc[j][2 * h + 1];
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
           }
         }
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
+        for (int kk = 0; kk < KEYS / 16; kk++) {
           // probabilities rounded to the cache's type: the second product's operand
           const uint32_t pa[4] = {Mma<E>::pack(sc[2 * kk][0], sc[2 * kk][1]), Mma<E>::pack(sc[2 * kk][2], sc[2 * kk][3]),
                                   Mma<E>::pack(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
 #pragma unroll
           for (int nd = 0; nd < HD / 8; nd += 2) {
             uint32_t bf[4];
-            ldsm_x4_t(bf, sV + tile_off<64>(kk * 16 + (lane % 8) + (mat % 2) * 8, nd + mat / 2));
+            ldsm_x4_t(bf, sV + tile_off<64>(koff + kk * 16 + (lane % 8) + (mat % 2) * 8, nd + mat / 2));
             Mma<E>::run(acc[nd], pa, bf[0], bf[1]);
             Mma<E>::run(acc[nd + 1], pa, bf[2], bf[3]);
           }

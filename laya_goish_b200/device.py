@@ -17,7 +17,6 @@ counterpart in the reference, which has no K/V cache.
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple
 
 import torch
@@ -25,61 +24,26 @@ import torch
 from . import _lib
 from ._lib import E_INVALID, E_TIMEOUT, LayaError, check
 
+try:
+    from . import _device
+except ImportError as e:
+    raise RuntimeError("_device.so is not built: run `python -m laya_goish_b200.build` (needs nvcc and g++)") from e
+
 PAGE = 64  # tokens per page
 MAX_TOP = 64
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 STATUS_TIMEOUT, STATUS_PAGE, STATUS_TOKEN, STATUS_ROWS = 1, 2, 4, 8
 
 
-_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without making a Stream object
-_current = torch._C._cuda_getDevice
-
-
 def _refuse(message: str):
     raise LayaError(E_INVALID, message)
 
 
-def _tensor(x, name: str, dim: int, dtype=None, device=None) -> None:
-    # plain tests: a message is only put together when one fails (a call costs a few microseconds)
+def _pages(x, name: str) -> None:
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
         _refuse(f"{name} must be a CUDA tensor")
-    if x.dim() != dim:
-        _refuse(f"{name} must have {dim} dimension(s)")
-    if dtype is not None and x.dtype is not dtype:
-        _refuse(f"{name} must be {dtype}")
-    if device is not None and x.device != device:
-        _refuse(f"{name} is on another device")
-    if x.requires_grad and torch.is_grad_enabled():
-        _refuse(f"{name} requires a gradient; the operators are forward only")
-
-
-def _flat(x, name: str, dtype, device) -> None:
-    _tensor(x, name, 1, dtype, device)
-    if not x.is_contiguous():
-        _refuse(f"{name} must be contiguous")
-
-
-def _rows(x, name: str) -> int:
-    """Row stride of a tensor whose rows (everything past dimension 0) are contiguous."""
-    shape, stride = x.shape, x.stride()
-    width = 1
-    for d in range(len(shape) - 1, 0, -1):
-        if shape[d] != 1 and stride[d] != width:
-            _refuse(f"the rows of {name} must be contiguous")
-        width *= shape[d]
-    return stride[0] if shape[0] > 1 else width
-
-
-def _call(device, fn, *args):
-    """Runs a library entry point with the tensors' device current, on its current stream."""
-    index = device.index
-    if _current() == index:
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream(index))
-    if rc < 0:
-        check(rc)
+    if x.dim() != 4:
+        _refuse(f"{name} must have 4 dimensions")
 
 
 def check_status(device: int = 0) -> None:
@@ -114,33 +78,7 @@ def page_plan(past, count, free_pages, tables, capacity: int, base: int = 0) -> 
     sequence order and are written into tables ([n, width] int32, in place;
     other entries stay as they are).  Rows are numbered through the sequences;
     positions start at base + past[i].  past, count: [n] int32; n <= 8192."""
-    _tensor(tables, "tables", 2, torch.int32)
-    dev = tables.device
-    n, width = tables.shape
-    _flat(past, "past", torch.int32, dev)
-    _flat(count, "count", torch.int32, dev)
-    _flat(free_pages, "free_pages", torch.int32, dev)
-    if past.shape[0] != n or count.shape[0] != n:
-        _refuse("past, count and tables must have one row per sequence")
-    if n and width > 1 and tables.stride(1) != 1:
-        _refuse("the rows of tables must be contiguous")
-    stride = tables.stride(0) if n > 1 else width
-    if stride < width:
-        _refuse("the rows of tables overlap")
-    if not 0 <= capacity < 1 << 31:
-        _refuse("capacity out of range")
-    if not 0 <= base < 1 << 31:
-        _refuse("base out of range")
-    # the outputs share one allocation, each on 16 bytes
-    a, c, m = -capacity % 4, 2 * (capacity % 2), (n + 1 + 3) // 4 * 4
-    slots, _, positions, _, seqs, _, offsets, _, lens, _, totals = torch.split_with_sizes(
-        tables.new_empty(4 * capacity + c + 2 * a + 2 * m + 4),
-        (2 * capacity, c, capacity, a, capacity, a, n + 1, m - n - 1, n, m - n, 4))
-    slots, totals = slots.view(torch.int64), totals.view(torch.int64)[:2]
-    _call(dev, _lib.lib().laya_page_plan, past.data_ptr(), count.data_ptr(), n, free_pages.data_ptr(),
-          free_pages.shape[0], base, tables.data_ptr(), stride, width, slots.data_ptr(), positions.data_ptr(),
-          seqs.data_ptr(), capacity, offsets.data_ptr(), lens.data_ptr(), totals.data_ptr())
-    return PagePlan(slots, positions, seqs, offsets, lens, totals)
+    return PagePlan(*_device.page_plan(past, count, free_pages, tables, capacity, base))
 
 
 class KVPages:
@@ -149,8 +87,10 @@ class KVPages:
     held token by token ([pages, 64, kv_heads, head_dim].permute(0, 2, 1, 3))."""
 
     def __init__(self, k, v):
-        _tensor(k, "k pages", 4)
-        _tensor(v, "v pages", 4, k.dtype, k.device)
+        _pages(k, "k pages")
+        _pages(v, "v pages")
+        if v.dtype != k.dtype or v.device != k.device:
+            _refuse("k and v pages must have the same type and device")
         if k.dtype not in (torch.float16, torch.bfloat16):
             _refuse("K/V pages must be F16 or BF16")
         if k.shape != v.shape:
@@ -179,7 +119,8 @@ class KVPages:
         self.pages, self.kv_heads, self.head_dim = pages, heads, hd
         self._c = _lib.KvPages(k.data_ptr(), v.data_ptr(), stride[0], stride[1], stride[2], pages, heads, hd,
                                TYPES[k.dtype])
-        self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
+        self._device = k.get_device()
 
 
 def kv_append(pages: KVPages, k, v, slots) -> None:
@@ -188,15 +129,7 @@ def kv_append(pages: KVPages, k, v, slots) -> None:
     distinct)."""
     if not isinstance(pages, KVPages):
         _refuse("pages must be KVPages")
-    _tensor(k, "k", 3, None, pages.device)
-    _tensor(v, "v", 3, k.dtype, pages.device)
-    _flat(slots, "slots", torch.int64, pages.device)
-    if k.dtype not in (pages.dtype, torch.float32):
-        _refuse("k and v must be of the pages' type or F32")
-    if k.shape != v.shape or tuple(k.shape) != (slots.shape[0], pages.kv_heads, pages.head_dim):
-        _refuse("k and v must be [rows, kv_heads, head_dim] with a slot per row")
-    _call(pages.device, _lib.lib().laya_kv_append, pages._ref, TYPES[k.dtype], k.data_ptr(), v.data_ptr(),
-          _rows(k, "k"), _rows(v, "v"), slots.data_ptr(), k.shape[0])
+    _device.kv_append(pages._at, pages._device, k, v, slots)
 
 
 def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, lens, offsets, max_q: int,
@@ -210,52 +143,8 @@ def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, l
     lse ([rows, heads] F32, optional) receives ln sum exp of the scores."""
     if not isinstance(pages, KVPages):
         _refuse("pages must be KVPages")
-    dev = pages.device
-    _tensor(q, "q", 3, pages.dtype, dev)
-    rows, heads, hd = q.shape
-    if hd != pages.head_dim:
-        _refuse("q and the pages have different head_dim")
-    if not heads or heads % pages.kv_heads:
-        _refuse("heads must be a multiple of kv_heads")
-    _flat(prefix_pages, "prefix_pages", torch.int32, dev)
-    _flat(lens, "lens", torch.int32, dev)
-    _flat(offsets, "offsets", torch.int32, dev)
-    _tensor(tables, "tables", 2, torch.int32, dev)
-    n, width = tables.shape
-    if lens.shape[0] != n or offsets.shape[0] != n + 1:
-        _refuse("lens, offsets and tables must fit the sequences")
-    if n and width > 1 and tables.stride(1) != 1:
-        _refuse("the rows of tables must be contiguous")
-    if not 0 <= prefix_len <= prefix_pages.shape[0] * PAGE:
-        _refuse("prefix_pages must hold prefix_len tokens")
-    if not 0 <= max_q < 1 << 31:
-        _refuse("max_q out of range")
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
-    if out is None:
-        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-    else:
-        _tensor(out, "out", 3, pages.dtype, dev)
-        if out.shape != q.shape:
-            _refuse("out must have q's shape")
-    if lse is not None:
-        _tensor(lse, "lse", 2, torch.float32, dev)
-        if tuple(lse.shape) != (rows, heads) or not lse.is_contiguous():
-            _refuse("lse must be contiguous [rows, heads]")
-    if _current() != dev.index:  # the workspace goes by the device that runs the call
-        with torch.cuda.device(dev):
-            return prefix_attention(q, pages, prefix_pages, prefix_len, tables, lens, offsets, max_q, scale, out, lse)
-    L = _lib.lib()
-    a = _lib.PrefixArgs(q.data_ptr(), _rows(q, "q"), rows, heads, offsets.data_ptr(), n, max_q,
-                        prefix_pages.data_ptr(), prefix_len, width, tables.data_ptr(),
-                        tables.stride(0) if n > 1 else width, lens.data_ptr(), scale, out.data_ptr(),
-                        _rows(out, "out"), None if lse is None else lse.data_ptr(), None, 0)
-    ref = ctypes.byref(a)
-    a.workspace_bytes = size = L.laya_prefix_attention_workspace(pages._ref, ref)
-    if size:
-        work = q.new_empty(size, dtype=torch.uint8)
-        a.workspace = work.data_ptr()
-    _call(dev, L.laya_prefix_attention, pages._ref, ref)
-    return out
+    return _device.prefix_attention(pages._at, pages._device, q, prefix_pages, prefix_len, tables, lens, offsets,
+                                    max_q, scale, out, lse)
 
 
 class TokenLogprobs(NamedTuple):
@@ -272,23 +161,4 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     """Log probabilities of tokens ([n, c] int32) under the rows of logits ([n,
     vocab] F32, F16 or BF16), the rows' entropy and lse, and the `top` (at most
     64) likeliest tokens.  Logits of -inf are tokens that are not there."""
-    _tensor(logits, "logits", 2)
-    dev = logits.device
-    if logits.dtype not in TYPES:
-        _refuse("logits must be F32, F16 or BF16")
-    n, vocab = logits.shape
-    if not vocab:
-        _refuse("empty vocabulary")
-    _tensor(tokens, "tokens", 2, torch.int32, dev)
-    if tokens.shape[0] != n:
-        _refuse("tokens must have a row per row of logits")
-    if not 0 <= top <= MAX_TOP:
-        _refuse("top must be 0..64")
-    c = tokens.shape[1]
-    logprobs, entropy, lse, top_lp, ids = torch.split_with_sizes(
-        logits.new_empty(n * (c + 2 + 2 * top), dtype=torch.float32), (n * c, n, n, n * top, n * top))
-    logprobs, top_lp, ids = logprobs.view(n, c), top_lp.view(n, top), ids.view(torch.int32).view(n, top)
-    _call(dev, _lib.lib().laya_token_logprobs, TYPES[logits.dtype], logits.data_ptr(), _rows(logits, "logits"), n,
-          vocab, tokens.data_ptr(), _rows(tokens, "tokens") if c else 0, c, top, logprobs.data_ptr(),
-          entropy.data_ptr(), lse.data_ptr(), ids.data_ptr(), top_lp.data_ptr())
-    return TokenLogprobs(logprobs, entropy, lse, ids, top_lp)
+    return TokenLogprobs(*_device.token_logprobs(logits, tokens, top))
