@@ -162,9 +162,13 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int capacity = (int)integer(a[4], "capacity", 0, INT32_MAX), base = (int)integer(a[5], "base", 0, INT32_MAX);
     c10::cuda::CUDAGuard guard(dev);
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor slots = empty({capacity}, at::kLong, dev), positions = empty({capacity}, at::kInt, dev),
-               seqs = empty({capacity}, at::kInt, dev), offsets = empty({n + 1}, at::kInt, dev),
-               lens = empty({n}, at::kInt, dev), totals = empty({2}, at::kLong, dev);
+    // one allocation, each output on 16 bytes (the offsets below are in 32-bit words)
+    const int64_t c4 = (capacity + 3ll) / 4 * 4, n4 = (n + 4) / 4 * 4;
+    at::Tensor all = empty({2 * c4 + n4 + 2}, at::kLong, dev), words = all.view(at::kInt);
+    auto part = [&](int64_t size, int64_t at) { return words.as_strided({size}, {1}, at); };
+    at::Tensor slots = all.as_strided({capacity}, {1}, 0), totals = all.as_strided({2}, {1}, 2 * c4 + n4),
+               positions = part(capacity, 2 * c4), seqs = part(capacity, 3 * c4), offsets = part(n + 1, 4 * c4),
+               lens = part(n, 4 * c4 + n4);
     check(laya_page_plan(ptr<int32_t>(past), ptr<int32_t>(count), size32(n, "sequences"), ptr<int32_t>(free_pages),
                          size32(free_pages.size(0), "free_pages"), base, ptr<int32_t>(tables), stride,
                          size32(width, "tables"), ptr<int64_t>(slots), ptr<int32_t>(positions), ptr<int32_t>(seqs),
@@ -282,9 +286,11 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int64_t xs = rows_of(x, "logits"), ts = c ? rows_of(tokens, "tokens") : 0;
     c10::cuda::CUDAGuard guard(dev);
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor logprobs = empty({n, c}, at::kFloat, dev), entropy = empty({n}, at::kFloat, dev),
-               lse = empty({n}, at::kFloat, dev), ids = empty({n, top}, at::kInt, dev),
-               top_lp = empty({n, top}, at::kFloat, dev);
+    at::Tensor all = empty({n * (c + 2 + 2 * top)}, at::kFloat, dev);
+    auto part = [&](const at::Tensor& t, int64_t size, int64_t at) { return t.as_strided({n, size}, {size, 1}, at); };
+    at::Tensor logprobs = part(all, c, 0), entropy = all.as_strided({n}, {1}, n * c),
+               lse = all.as_strided({n}, {1}, n * (c + 1)), top_lp = part(all, top, n * (c + 2)),
+               ids = part(all.view(at::kInt), top, n * (c + 2 + top));
     check(laya_token_logprobs(type_code(type), ptr(x), xs, size32(n, "rows"), size32(vocab, "vocabulary"),
                               ptr<int32_t>(tokens), ts, size32(c, "tokens"), top, ptr<float>(logprobs),
                               ptr<float>(entropy), ptr<float>(lse), ptr<int32_t>(ids), ptr<float>(top_lp),
