@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   int* off = plan_sm;          // [n + 1] first rows, cut at the capacity
   int* pg = off + n + 1;       // [n] first free page, cut at n_free
   int* pst = pg + n;           // [n] past
-  __shared__ long long wsum[2][kPlanThreads / 32];
+  __shared__ long long wsum[2][kPlanThreads / 32 + 1];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   // sizes into shared memory, coalesced and four loads at a time
 #pragma unroll 4
@@ -103,16 +103,29 @@ __global__ void __launch_bounds__(kPlanThreads)
     wsum[1][warp] = ep;
   }
   __syncthreads();
-  long long bt = et - st, bp = ep - sp, all_t = 0, all_p = 0;
+  if (warp == 0) {  // exclusive sums of the warps, and the totals behind them
+    const long long t0 = lane < kPlanThreads / 32 ? wsum[0][lane] : 0, p0 = lane < kPlanThreads / 32 ? wsum[1][lane] : 0;
+    long long t = t0, q = p0;
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 32; w++) {
-    if (w < warp) {
-      bt += wsum[0][w];
-      bp += wsum[1][w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, t, o), y = __shfl_up_sync(0xffffffffu, q, o);
+      if (lane >= o) {
+        t += x;
+        q += y;
+      }
     }
-    all_t += wsum[0][w];
-    all_p += wsum[1][w];
+    if (lane < kPlanThreads / 32) {
+      wsum[0][lane] = t - t0;
+      wsum[1][lane] = q - p0;
+    }
+    if (lane == 31) {
+      wsum[0][kPlanThreads / 32] = t;
+      wsum[1][kPlanThreads / 32] = q;
+    }
   }
+  __syncthreads();
+  long long bt = et - st + wsum[0][warp], bp = ep - sp + wsum[1][warp];
+  const long long all_t = wsum[0][kPlanThreads / 32], all_p = wsum[1][kPlanThreads / 32];
   for (int i = i0; i < i1; i++) {
     const int c = off[i], f = pg[i];
     off[i] = (int)min(bt, (long long)capacity);
@@ -154,8 +167,11 @@ __global__ void __launch_bounds__(kPlanThreads)
       }
       i = lo;
     }
+    // places fit 32 unsigned bits: past and count are below 2^31
     long long sl[4];
     int po[4], se[4];
+    unsigned known = 0xffffffffu;  // page index that `page` is of
+    int page = -1;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const long long t = t0 + e;
@@ -163,18 +179,24 @@ __global__ void __launch_bounds__(kPlanThreads)
       po[e] = 0;
       se[e] = -1;
       if (t < total) {
-        while (off[i + 1] <= t) i++;  // ends: off[n] = total > t
-        const long long u = (long long)pst[i] + (t - off[i]);
-        const long long b = u / 64, a = b - ((long long)pst[i] + 63) / 64;
-        int page = -1;
-        if (b < width) {
-          if (a < 0)
-            page = tables[(long long)i * tstride + b];
-          else if (a < n_free - pg[i])
-            page = free_pages[pg[i] + a];
+        if (off[i + 1] <= t) {
+          while (off[i + 1] <= t) i++;  // ends: off[n] = total > t
+          known = 0xffffffffu;
+        }
+        const unsigned u = (unsigned)pst[i] + (unsigned)((int)t - off[i]), b = u / 64;
+        if (b != known) {
+          const unsigned have = ((unsigned)pst[i] + 63u) / 64;
+          known = b;
+          page = -1;
+          if (b < (unsigned)width) {
+            if (b < have)
+              page = tables[(long long)i * tstride + b];
+            else if (b - have < (unsigned)(n_free - pg[i]))
+              page = free_pages[pg[i] + (int)(b - have)];
+          }
         }
         if (page >= 0) sl[e] = (long long)page * 64 + (u & 63);
-        po[e] = (int)(base + u);
+        po[e] = (int)((unsigned)base + u);
         se[e] = i;
       }
     }
