@@ -55,7 +55,7 @@ struct PfxParams {
   int sp, ss;     // most prefix splits of a row (0: no prefix), own-key splits
   int q_tiles;    // row tiles per sequence (own keys) or over all rows (prefix)
   // tensor-core prefix kernel (chunk > 0): its units (kv head, unit_tok tokens)
-  // are `steps` key steps each, cut into runs of `chunk` steps over all units
+  // are `steps` pages each, cut into runs of `chunk` pages over all units
   int chunk, steps, unit_tok, n_units;
   int pages;      // pages of the cache
   unsigned* status;
@@ -140,7 +140,7 @@ struct Unit {
   static constexpr int PW = HD == 256 ? 3 : 2;
   static constexpr int NW = SPLITK ? 2 * PW : 4;
   static constexpr int KEYS = SPLITK ? 32 : 64;  // of a page per warp
-  static constexpr int THREADS = 32 * (NW + 1);
+  static constexpr int THREADS = 32 * NW;
   static constexpr int CTAS = HD == 256 ? 1 : HD == 128 && !SPLITK ? 2 : 3;  // per SM
   static constexpr int OFF_Q = S * STAGE;  // [HD / 64][ROWS][128 B]
   static constexpr int OFF_BAR = OFF_Q + ROWS * HD * 2;
@@ -152,8 +152,8 @@ struct Unit {
 
 // Attention of a tile of query rows over a list of whole 64-token pages with
 // mma.sync m16n8k16, for few rows per key list, where the K/V bytes bound it.
-// A producer warp streams each page's K and V (128-byte swizzled boxes) into
-// a ring; NW consumer warps compute.
+// Each page's K and V come by TMA (128-byte swizzled boxes) into a ring; the
+// first warp of those that share a stage fills it again when they are done.
 //   SPLITK: 16 rows; warps 2 w and 2 w + 1 take halves of pages w, w + PW, ...
 //           with online softmaxes of their own, and the warps' states are joined
 //           in shared memory.
@@ -165,7 +165,7 @@ struct Unit {
 // numbers, pages, partials, output) is hidden by other units: small rings,
 // two or three CTAs per SM (measured in DESIGN's table).
 template <typename E, int HD, bool SPLITK, bool OWN>
-__global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::CTAS)
+__global__ void __maxnreg__((HD == 256 ? 255 : 168))
     prefix_unit_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const PfxParams p) {
   using C = Unit<HD, SPLITK>;
@@ -186,9 +186,13 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
   u /= p.KV;
   const int tile = u % p.q_tiles, b = u / p.q_tiles;
   const int* list = OWN ? p.tables + (long long)b * p.tstride : p.prefix_pages;
+  // The warps that share pages: SPLITK pairs (pages w, w + PW, ...), else all.
+  constexpr int STEP = SPLITK ? C::PW : 1;
+  const int first = SPLITK ? warp >> 1 : 0;
+  const bool leads = (SPLITK ? (warp & 1) == 0 : warp == 0);
   // the first page numbers, before the sizes that say how many count
   const int list_len = OWN ? p.width : (p.prefix_len + 63) / 64;
-  int ids = warp == C::NW && splits == 1 && lane < list_len ? list[lane] : 0;
+  int ids = splits == 1 && lane < list_len ? list[lane] : 0;
 
   Seq sq;
   if (OWN) {
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
   const int f0 = tile * ROWS, n_flat = sq.nq * p.G;
   const int nr = min(ROWS, n_flat - f0);  // rows of this tile
   if (nr <= 0) {
-    pdl_wait();  // every CTA: this kernel ends after the one before it
+    if (OWN && blockIdx.x == 0) pdl_wait();  // as at the end
     return;
   }
   // keys that row f sees: OWN len - nq + token + 1 (may be < 1), else all
@@ -241,40 +245,32 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 
-  if (warp == C::NW) {
-    int i = 0;
-    for (; i < np; i++) {
-      if (i % 32 == 0 && (i || splits > 1)) ids = p0 + i + lane < n_pages ? list[p0 + i + lane] : 0;
-      const int page = __shfl_sync(0xffffffffu, ids, i % 32);
+  if (splits > 1) ids = p0 + lane < n_pages ? list[p0 + lane] : 0;
+  // Page i of this CTA's into stage i % S: lane 0 of a leading warp, which its
+  // stage's warps have left (or that holds nothing yet).
+  auto fill = [&](int i) {
+    const int page = i < 32 ? __shfl_sync(0xffffffffu, ids, i) : list[p0 + i];
+    if (lane == 0) {
       const int st = i % C::S;
-      int ok = 1;
-      if (lane == 0) ok = mbar_wait(&empty[st], ((i / C::S) & 1) ^ 1, kBudget);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      if (lane == 0) {
-        const bool in = page >= 0 && page < p.pages;
-        page_ok[st] = in;
-        if (in) {
-          uint8_t* dst = sm + st * C::STAGE;
-          mbar_expect_tx(&full[st], C::STAGE);
+      const bool in = page >= 0 && page < p.pages;
+      page_ok[st] = in;
+      if (in) {
+        uint8_t* dst = sm + st * C::STAGE;
+        mbar_expect_tx(&full[st], C::STAGE);
 #pragma unroll
-          for (int hb = 0; hb < HD / 64; hb++) {
-            tma_load_4d(dst + hb * 8192, &tk, &full[st], hb * 64, 0, kvh, page);
-            tma_load_4d(dst + C::PAGE + hb * 8192, &tv, &full[st], hb * 64, 0, kvh, page);
-          }
-        } else {
-          atomicOr(p.status, LAYA_STATUS_PAGE);
-          mbar_arrive(&full[st]);
+        for (int hb = 0; hb < HD / 64; hb++) {
+          tma_load_4d(dst + hb * 8192, &tk, &full[st], hb * 64, 0, kvh, page);
+          tma_load_4d(dst + C::PAGE + hb * 8192, &tv, &full[st], hb * 64, 0, kvh, page);
         }
+      } else {
+        atomicOr(p.status, LAYA_STATUS_PAGE);
+        mbar_arrive(&full[st]);
       }
     }
-    if (lane == 0) {
-      if (i < np) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
-      // no copy is in flight when the ring is reused or the CTA ends
-      for (int x = max(0, i - C::S); x < i; x++)
-        if (!mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget)) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
-    }
-    __syncwarp();
-  } else if (warp < C::NW) {
+  };
+  if (leads)
+    for (int i = first; i < min(np, C::S); i += STEP) fill(i);
+  {
     // visible keys of this thread's two rows
     int vis[2];
 #pragma unroll
@@ -282,10 +278,12 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
       vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
     constexpr int KEYS = C::KEYS;
     const int koff = SPLITK ? (warp & 1) * 32 : 0;  // this warp's first key of a page
-    for (int i = SPLITK ? warp >> 1 : 0; i < np; i += SPLITK ? C::PW : 1) {
+    for (int i = first; i < np; i += STEP) {
       const int st = i % C::S;
       if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (i / C::S) & 1, kBudget))) {
         if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+        // give the copies that are still on their way as long again
+        for (int x = i; x < min(np, i + C::S); x += STEP) mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget);
         break;
       }
       const uint8_t* sK = sm + st * C::STAGE;
@@ -370,7 +368,16 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      if (i + C::S < np) {  // the stage's next page, once its warps have left it
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (leads) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], (i / C::S) & 1, kBudget))) {
+            if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+            break;
+          }
+          fill(i + C::S);
+        }
+      }
     }
   }
   // ---- the tile's results
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
     // join the warps' states through the (drained) ring: [NW][16][HD + 2]
     __syncthreads();
     float* comb = reinterpret_cast<float*>(sm);
-    if (warp < C::NW) {
+    {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         float* cw = comb + (warp * 16 + g + 8 * h) * (HD + 2);
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
       }
     }
   } else {
-    if (warp < 4) {
+    {
 #pragma unroll
       for (int hh = 0; hh < 2; hh++) {
         const int r = wr + g + 8 * hh;
@@ -448,8 +455,9 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
     }
   }
   // The join kernel's griddepcontrol.wait has to cover the prefix kernel, too:
-  // this one ends after it.
-  if (OWN) pdl_wait();
+  // one CTA ends after it, and with that this kernel does (all of them would
+  // keep their places on the SMs).
+  if (OWN && blockIdx.x == 0) pdl_wait();
 }
 
 // ------------------------------------------------------------ prefix, many rows
@@ -457,52 +465,56 @@ __global__ void __launch_bounds__(Unit<HD, SPLITK>::THREADS, Unit<HD, SPLITK>::C
 // For more than 16 rows per kv head the prefix is a product of matrices and
 // runs on the tcgen05 tensor cores.  A unit is one kv head and NT tiles of
 // 128 query rows (a tile: TT = 128 / G tokens, row = token * G + head of the
-// group); its keys go by in steps of 128 (two pages):
-//   S = Q K^T   (M 128, N 128 into TMEM),  P = 2^(S - ref),  O += P V
+// group); its keys go by a page (64) at a time:
+//   S = Q K^T   (M 128, N 64, into one of the tile's two score buffers in TMEM),
+//   P = 2^(S - ref),  O += P V
 // with P written back over S in TMEM as the next product's A operand.
-//   warp 0        TMA: Q, then K and V of each step into one ring of stages
-//   warp 1        one thread issues the products; while one tile's softmax
-//                 runs, the other tile's products do
+//   warp 0        TMA: Q, then K and V of each page into one ring of stages
+//   warp 1        one thread issues the products, the scores two pages ahead:
+//                 the softmax of a page does not wait for its scores
 //   warps 4 ..    softmax, four warps per tile, thread = row = TMEM lane.  O is
 //                 rescaled in TMEM only when a row's maximum passes its
 //                 reference by 2^15 (P stays below 2^15; ref = max - 7 keeps
 //                 small probabilities out of F16's subnormals).
-// Two tiles per unit halve the K/V bytes from L2 per row and keep both the
-// tensor cores (1024 cycles per tile and step at head_dim 128) and the
-// exponentials (16384 at 16 per cycle: 1024 cycles) busy; head_dim 256 has
-// room for one tile in TMEM.
-// The steps of all units, one unit after the other, are cut into equal runs,
+// Per page and two tiles at head_dim 128 the tensor cores need 1024 cycles (the
+// scores' N = 64 makes shared memory their limit: 1280) and the exponentials
+// (16384 at 16 per cycle) 1024, so both have to run at once.  With one score
+// buffer of 128 keys per tile, scores issued behind the page's P V, they took
+// turns (51% and 52% busy; eight softmax warps per tile changed nothing).
+// Two tiles per unit halve the K/V bytes from L2 per row; head_dim 256 has room
+// for one tile in TMEM.
+// The pages of all units, one unit after the other, are cut into equal runs,
 // one per CTA, so the GPU is evenly loaded whatever the sizes; a unit cut by a
 // run's end leaves one partial result per run (prefix_splits).
 // The last page's rows past the prefix come as zeros from a tensor map that
 // ends there, so nothing stale meets a probability of 0; pages outside the
-// cache, and a step's missing second page, are loaded out of bounds (zeros).
-template <int HD>
+// cache are loaded out of bounds (zeros) and masked.
+template <int HD, int NT_>
 struct Ptc {
-  static constexpr int NT = HD == 256 ? 1 : 2;
+  static constexpr int NT = NT_;
   static constexpr int Q_TILE = 128 * HD * 2;  // [HD / 64][128 rows][128 B]
-  static constexpr int STAGE = 128 * HD * 2;   // K or V of a step, the same layout
-  static constexpr int NS = HD == 64 ? 9 : HD == 128 ? 4 : 2;
+  static constexpr int STAGE = 64 * HD * 2;    // K or V of a page: [HD / 64][64 rows][128 B]
+  static constexpr int NS = HD == 256 ? 4 : HD == 64 ? 10 : NT == 1 ? 6 : 5;
   static constexpr int OFF_RING = NT * Q_TILE;
-  static constexpr int OFF_OUT = OFF_RING + NS * STAGE;  // 32 x 32 F32 per softmax warp, for coalesced partials
-  static constexpr int OFF_BAR = OFF_OUT + NT * 4 * 4096;
-  static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 4 * NT) * 8 + 16 + 1024;
+  static constexpr int OFF_OUT = OFF_RING + NS * STAGE;  // 1 KB per softmax warp: 32 rows x 8 F32, coalesced partials
+  static constexpr int OFF_BAR = OFF_OUT + NT * 4 * 1024;
+  static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 7 * NT) * 8 + 16 + 1024;
   static constexpr int THREADS = 128 + NT * 128;
-  // NT = 2: 168 registers per thread at launch; the first warpgroup's surplus
-  // goes to the softmax threads, which hold a row of 128 scores.
-  static constexpr int REG_LOW = 88, REG_HIGH = 208;
-  static_assert(REG_LOW + 2 * REG_HIGH <= 3 * 168, "register split");
-  static constexpr int COLS = 512;
-  static constexpr int S_COL = 0, O_COL = NT * 128;  // tile t: S at 128 t, O at O_COL + HD t
+  static constexpr int COLS = NT * (128 + HD) <= 256 ? 256 : 512;
+  static constexpr int S_COL = 0, O_COL = NT * 128;  // tile t: S at 128 t and 128 t + 64, O at O_COL + HD t
   static_assert(O_COL + NT * HD <= COLS, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
-struct Run {  // a CTA's part of a unit
+// Per thread: leaves an SM quarter, beside three of these warps, room for one of
+// the own-keys kernel's.
+constexpr int kTcRegs = 112;
+
+struct Run {  // a CTA's part of a unit: pages s0 .. s1 - 1
   int kvh, tok0, s0, s1, plane, tiles;
 };
 
-// Part i = 0, 1, ... of CTA c's run [c * chunk, (c + 1) * chunk) of key steps.
+// The next part of a CTA's run [c * chunk, (c + 1) * chunk) of pages.
 __device__ __forceinline__ bool run_part(const PfxParams& p, long long& at, long long end, int nt, int tt, Run& r) {
   if (at >= end) return false;
   const long long u = at / p.steps;
@@ -517,13 +529,12 @@ __device__ __forceinline__ bool run_part(const PfxParams& p, long long& at, long
   return true;
 }
 
-template <typename E, int HD>
-__global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
+template <typename E, int HD, int NT>
+__global__ void __maxnreg__(kTcRegs)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tv_last,
                      const PfxParams p) {
-  using C = Ptc<HD>;
-  constexpr int NT = C::NT;
+  using C = Ptc<HD, NT>;
   extern __shared__ uint8_t pt_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = sm + C::OFF_RING;
@@ -531,11 +542,12 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
   uint64_t* empty = full + C::NS;                                 // [NS]
   uint64_t* q_full = empty + C::NS;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;   // [NT] scores of a step
-  uint64_t* p_full = s_full + NT;   // [NT] probabilities of a step (4 warps)
-  uint64_t* o_full = p_full + NT;   // [NT] O of a part complete
-  uint64_t* o_empty = o_full + NT;  // [NT] O read (4 warps)
-  uint64_t* fin = o_empty + NT;     // all products of the CTA
+  uint64_t* s_full = q_empty + 1;      // [NT][2] scores of a page
+  uint64_t* p_full = s_full + 2 * NT;  // [NT][2] probabilities of a page (4 warps)
+  uint64_t* o_done = p_full + 2 * NT;  // [NT] one phase per page's P V
+  uint64_t* o_full = o_done + NT;      // [NT] O of a part complete
+  uint64_t* o_empty = o_full + NT;     // [NT] O read (4 warps)
+  uint64_t* fin = o_empty + NT;        // all products of the CTA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = p.G, TT = 128 / G;
@@ -554,8 +566,11 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
     mbar_init(q_empty, 1);
     mbar_init(fin, 1);
     for (int t = 0; t < NT; t++) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&s_full[2 * t + i], 1);
+        mbar_init(&p_full[2 * t + i], 4);
+      }
+      mbar_init(&o_done[t], 1);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_empty[t], 4);
     }
@@ -572,7 +587,6 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
   const uint32_t tbase = *tmem_slot;
   long long at = (long long)blockIdx.x * p.chunk;
   const long long end = min(at + p.chunk, (long long)p.n_units * p.steps);
-  const int n_pages = (p.prefix_len + 63) / 64;
   unsigned bad = 0;
   bool live = true;  // false once a wait ran out: every role then leaves its loops
   auto wait = [&](uint64_t* b, uint32_t parity) {
@@ -582,7 +596,6 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
   Run r;
 
   if (warp < 4) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_LOW));
     if (warp == 0) {
       if (lane == 0) {
         int g = 0, k = 0;  // stages, parts
@@ -594,15 +607,13 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
             for (int hb = 0; hb < HD / 64; hb++)
               tma_load_3d(sm + t * C::Q_TILE + hb * 16384, &tq, q_full, hb * 64, r.kvh * G, r.tok0 + t * TT);
           k++;
+          int next = p.prefix_pages[r.s0];
           for (int s = r.s0; s < r.s1 && live; s++) {
-            int page[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              page[h] = 2 * s + h < n_pages ? p.prefix_pages[2 * s + h] : p.pages;
-              if (page[h] < 0 || page[h] >= p.pages) {
-                if (2 * s + h < n_pages) bad |= LAYA_STATUS_PAGE;
-                page[h] = p.pages;  // out of bounds: zeros
-              }
+            int page = next;
+            if (s + 1 < r.s1) next = p.prefix_pages[s + 1];
+            if (page < 0 || page >= p.pages) {
+              bad |= LAYA_STATUS_PAGE;
+              page = p.pages;  // out of bounds: zeros
             }
 #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
@@ -610,13 +621,10 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
               if (!wait(&empty[st], ((g / C::NS) & 1) ^ 1)) break;
               g++;
               mbar_expect_tx(&full[st], C::STAGE);
+              const void* map = kv == 0 ? &tk : s == p.steps - 1 ? &tv_last : &tv;
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const void* map = kv == 0 ? &tk : 2 * s + h == n_pages - 1 ? &tv_last : &tv;
-#pragma unroll
-                for (int hb = 0; hb < HD / 64; hb++)
-                  tma_load_4d(ring + st * C::STAGE + hb * 16384 + h * 8192, map, &full[st], hb * 64, 0, r.kvh, page[h]);
-              }
+              for (int hb = 0; hb < HD / 64; hb++)
+                tma_load_4d(ring + st * C::STAGE + hb * 8192, map, &full[st], hb * 64, 0, r.kvh, page);
             }
           }
         }
@@ -628,54 +636,57 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
       }
     } else if (warp == 1) {
       if (elect_one()) {
-        constexpr bool BF = sizeof(E) == 2 && !__is_same(E, half);
-        const uint32_t id_s = BF ? idesc_bf16_f32(128, 128) : idesc_f16_f32(128, 128);
+        constexpr bool BF = !__is_same(E, half);
+        const uint32_t id_s = BF ? idesc_bf16_f32(128, 64) : idesc_f16_f32(128, 64);
         const uint32_t id_o = (BF ? idesc_bf16_f32(128, HD) : idesc_f16_f32(128, HD)) | (1u << 16);  // V MN-major
         int g = 0, k = 0;
-        int steps_t[NT] = {}, parts_t[NT] = {};
+        int steps_t[NT] = {}, parts_t[NT] = {};  // pages with P V issued, parts, of each tile
         while (live && run_part(p, at, end, NT, TT, r)) {
           if (!wait(q_full, k & 1)) break;
           k++;
           const int ns = r.s1 - r.s0;
-          // scores of step j (ring stage g + 2 j) for tile t
+          // scores of the part's page j (ring stage g + 2 j) for tile t
           auto scores = [&](int j, int t) {
-            const int x = g + 2 * j, st = x % C::NS;
+            const int x = g + 2 * j, st = x % C::NS, buf = (steps_t[t] + (j > 1 ? 1 : j)) & 1;
             if (!wait(&full[st], (x / C::NS) & 1)) return;
             tc_fence_after();
-            const uint8_t* q = sm + t * C::Q_TILE;
-            const uint8_t* kk0 = ring + st * C::STAGE;
+            // descriptors of the later k-steps: the start address field plus a constant
+            const uint64_t qd = sw128_desc(smem_u32(sm + t * C::Q_TILE));
+            const uint64_t kd = sw128_desc(smem_u32(ring + st * C::STAGE));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++)
-              umma_f16(tbase + C::S_COL + t * 128, sw128_desc(smem_u32(q + (kk >> 2) * 16384 + (kk & 3) * 32)),
-                       sw128_desc(smem_u32(kk0 + (kk >> 2) * 16384 + (kk & 3) * 32)), id_s, kk > 0 ? 1u : 0u);
-            umma_commit(&s_full[t]);
+              umma_f16(tbase + C::S_COL + t * 128 + buf * 64, qd + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                       kd + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[2 * t + buf]);
             if (t == r.tiles - 1) {
               umma_commit(&empty[st]);
               if (j == ns - 1) umma_commit(q_empty);
             }
           };
-          for (int t = 0; t < r.tiles; t++) scores(0, t);
+          for (int j = 0; j < 2 && j < ns; j++)
+            for (int t = 0; t < r.tiles; t++) scores(j, t);
           for (int j = 0; j < ns && live; j++) {
             const int x = g + 2 * j + 1, st = x % C::NS;
             for (int t = 0; t < r.tiles; t++) {
+              const int buf = steps_t[t] & 1;
               if (j == 0) wait(&o_empty[t], (parts_t[t] & 1) ^ 1);
               wait(&full[st], (x / C::NS) & 1);
-              if (!wait(&p_full[t], steps_t[t] & 1)) break;
+              if (!wait(&p_full[2 * t + buf], (steps_t[t] >> 1) & 1)) break;
               steps_t[t]++;
               tc_fence_after();
-              const uint8_t* v = ring + st * C::STAGE;
+              const uint64_t vd = sw128_mn_desc(smem_u32(ring + st * C::STAGE), 8192, 1024);
 #pragma unroll
-              for (int kk = 0; kk < 8; kk++)
-                umma_f16_ta(tbase + C::O_COL + t * HD, tbase + C::S_COL + t * 128 + kk * 8,
-                            sw128_mn_desc(smem_u32(v + kk * 2048), 16384, 1024), id_o, (j > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < 4; kk++)
+                umma_f16_ta(tbase + C::O_COL + t * HD, tbase + C::S_COL + t * 128 + buf * 64 + kk * 8,
+                            vd + kk * (2048 >> 4), id_o, (j > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&o_done[t]);
               if (t == r.tiles - 1) umma_commit(&empty[st]);
               if (j == ns - 1) {
                 umma_commit(&o_full[t]);
                 parts_t[t]++;
-              } else {
-                // over this tile's P: products run in the order of issue
-                scores(j + 1, t);
               }
+              // over the P just used: products run in the order of issue
+              if (j + 2 < ns) scores(j + 2, t);
             }
           }
           g += 2 * ns;
@@ -684,59 +695,62 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
         umma_commit(fin);
         mbar_wait(fin, 0, kBudget);
       }
-    }  // warps 2 and 3 only lend their registers
+    }  // warps 2 and 3: nothing (a softmax warp's lanes go by warp % 4)
   } else {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_HIGH));
     const int t = (warp - 4) / 4, quarter = warp % 4, row = quarter * 32 + lane;
     const uint32_t tl = tbase + ((uint32_t)(quarter * 32) << 16);
     const uint32_t tS = tl + C::S_COL + t * 128, tO = tl + C::O_COL + t * HD;
-    int step = 0, part = 0;
+    int step = 0, part = 0;  // of this tile
     while (live && run_part(p, at, end, NT, TT, r)) {
       if (t >= r.tiles) continue;
       const int tok = r.tok0 + t * TT + row / G, h = r.kvh * G + row % G;
       const bool valid = row < TT * G && tok < p.rows;
       const bool busy = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers' count
       float mref = -INFINITY, l = 0.f;
+      int next = __ldg(p.prefix_pages + r.s0);
       for (int s = r.s0; s < r.s1; s++, step++) {
-        // pages of this step that are in the cache
-        int lim = min(128, p.prefix_len - s * 128);
-        const int pg0 = __ldg(p.prefix_pages + 2 * s);
-        const int pg1 = 2 * s + 1 < n_pages ? __ldg(p.prefix_pages + 2 * s + 1) : 0;
-        const bool ok0 = pg0 >= 0 && pg0 < p.pages, ok1 = pg1 >= 0 && pg1 < p.pages;
-        live = __all_sync(0xffffffffu, wait(&s_full[t], step & 1));
+        const int page = next, buf = step & 1;
+        if (s + 1 < r.s1) next = __ldg(p.prefix_pages + s + 1);
+        // keys of the page that are there
+        const int seen = page >= 0 && page < p.pages ? min(64, p.prefix_len - s * 64) : 0;
+        live = __all_sync(0xffffffffu, wait(&s_full[2 * t + buf], (step >> 1) & 1));
         if (!live) break;
         tc_fence_after();
         if (busy) {
-          uint32_t v[128];
+          uint32_t v[64];
           __syncwarp();
-#pragma unroll
-          for (int c = 0; c < 4; c++) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+          tmem_ld32(tS + buf * 64, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld32(tS + buf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tmem_ld_wait();
-          if (lim < 128 || !ok0 || !ok1) {
+          if (seen < 64) {
 #pragma unroll
-            for (int c = 0; c < 128; c++)
-              if (c >= lim || !(c < 64 ? ok0 : ok1)) v[c] = 0xff800000u;
+            for (int c = 0; c < 64; c++)
+              if (c >= seen) v[c] = 0xff800000u;
           }
           float m4[4];
 #pragma unroll
           for (int c = 0; c < 4; c++) m4[c] = __uint_as_float(v[c]);
 #pragma unroll
-          for (int c = 4; c < 128; c++) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(v[c]));
+          for (int c = 4; c < 64; c++) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(v[c]));
           // the scale is positive, so the maximum commutes with it
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
           const float nref = mx > mref + 15.f ? mx - 7.f : mref;
           if (s > r.s0 && __any_sync(0xffffffffu, nref != mref)) {
-            // this step's scores were issued after the last O += P V, so that one is complete
+            // These scores were issued behind the P V before the last one, so
+            // o_done is in the last one's phase or past it.
+            live = __all_sync(0xffffffffu, wait(&o_done[t], (step - 1) & 1));
+            if (!live) break;
+            tc_fence_after();
             const float corr = nref != mref ? ex2(mref - nref) : 1.f;
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-              uint32_t o[32];
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; c++) {
+              uint32_t o[16];
               __syncwarp();
-              tmem_ld32(tO + c * 32, o);
+              tmem_ld16(tO + c * 16, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(tO + c * 32, o);
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st16(tO + c * 16, o);
             }
             l *= corr;
           }
@@ -748,12 +762,12 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
           asm("mov.b64 %0, {%1, %1};" : "=l"(acc2[0]) : "f"(0.f));
           acc2[1] = acc2[0];
 #pragma unroll
-          for (int b = 0; b < 2; b++) {
-            uint32_t w[32];
+          for (int q = 0; q < 2; q++) {
+            uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
+            for (int c = 0; c < 32; c += 2) {
               unsigned long long x2, e2, p2;
-              asm("mov.b64 %0, {%1, %2};" : "=l"(x2) : "r"(v[64 * b + c]), "r"(v[64 * b + c + 1]));
+              asm("mov.b64 %0, {%1, %2};" : "=l"(x2) : "r"(v[32 * q + c]), "r"(v[32 * q + c + 1]));
               asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e2) : "l"(x2), "l"(sc2), "l"(nm2));
               float e0, e1;
               asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(e2));
@@ -765,7 +779,7 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
               w[c >> 1] = Mma<E>::pack(e0, e1);
             }
             __syncwarp();
-            tmem_st32(tS + 32 * b, w);
+            tmem_st16(tS + buf * 64 + q * 16, w);
           }
           float l4[4];
           asm("mov.b64 {%0, %1}, %2;" : "=f"(l4[0]), "=f"(l4[1]) : "l"(acc2[0]));
@@ -775,8 +789,9 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
       }
+      if (!live) break;
       live = __all_sync(0xffffffffu, wait(&o_full[t], part & 1));
       if (!live) break;
       part++;
@@ -785,32 +800,38 @@ __global__ void __launch_bounds__(Ptc<HD>::THREADS, 1)
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const size_t th = (size_t)tok * p.H + h, rowsH = (size_t)p.rows * p.H;
         if (valid) p.part_l[r.plane * rowsH + th] = mref == -INFINITY ? -INFINITY : mref - log2f(inv);
-        // a lane holds a row; through shared memory 8 lanes write 128 bytes of one
-        // (16-byte pieces, piece j of row i at j ^ (i % 8))
-        uint4* stage = reinterpret_cast<uint4*>(sm + C::OFF_OUT) + (warp - 4) * 256;
+        // A lane holds a row; through shared memory two lanes write 32 bytes of one
+        // (16-byte pieces, piece j of row i at j ^ (i / 4 % 2)).
+        uint4* stage = reinterpret_cast<uint4*>(sm + C::OFF_OUT) + (warp - 4) * 64;
         const int mine = valid ? (int)th : -1;
-        int rows8[8];  // the rows lane / 8, lane / 8 + 4, ... that this lane writes
+        int rows2[2];  // the rows lane / 2 and lane / 2 + 16, which this lane writes
 #pragma unroll
-        for (int i = 0; i < 8; i++) rows8[i] = __shfl_sync(0xffffffffu, mine, i * 4 + lane / 8);
-#pragma unroll
+        for (int i = 0; i < 2; i++) rows2[i] = __shfl_sync(0xffffffffu, mine, i * 16 + lane / 2);
+        float* dst = p.part_o + r.plane * rowsH * HD + (lane & 1) * 4;
+#pragma unroll 1
         for (int c = 0; c < HD / 32; c++) {
           uint32_t o[32];
           __syncwarp();
           tmem_ld32(tO + c * 32, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            stage[lane * 8 + (j ^ (lane & 7))] =
-                make_uint4(__float_as_uint(__uint_as_float(o[4 * j]) * inv), __float_as_uint(__uint_as_float(o[4 * j + 1]) * inv),
-                           __float_as_uint(__uint_as_float(o[4 * j + 2]) * inv),
-                           __float_as_uint(__uint_as_float(o[4 * j + 3]) * inv));
-          __syncwarp();
+          for (int b = 0; b < 4; b++) {
+            __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int row = i * 4 + lane / 8;
-            const uint4 x = stage[row * 8 + ((lane & 7) ^ (row & 7))];
-            if (rows8[i] >= 0)
-              *reinterpret_cast<uint4*>(p.part_o + (r.plane * rowsH + rows8[i]) * HD + c * 32 + (lane & 7) * 4) = x;
+            for (int j = 0; j < 2; j++) {
+              const uint32_t* x = o + 8 * b + 4 * j;
+              stage[lane * 2 + (j ^ (lane >> 2 & 1))] = make_uint4(
+                  __float_as_uint(__uint_as_float(x[0]) * inv), __float_as_uint(__uint_as_float(x[1]) * inv),
+                  __float_as_uint(__uint_as_float(x[2]) * inv), __float_as_uint(__uint_as_float(x[3]) * inv));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int at_row = i * 16 + lane / 2;
+              const uint4 x = stage[at_row * 2 + ((lane & 1) ^ (at_row >> 2 & 1))];
+              if (rows2[i] >= 0)
+                *reinterpret_cast<uint4*>(dst + (size_t)rows2[i] * HD + c * 32 + b * 8) = x;
+            }
           }
         }
       }
@@ -890,8 +911,9 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p, int
 struct Shape {
   int sp, ss;      // most prefix splits of a row, own-key splits
   bool own_split;  // own keys: 16-row tiles with the pages shared by the warps
-  int own_tiles;
+  int own_tiles, pre_tiles;
   bool tc;         // prefix on the tensor cores (else one 16-row tile per kv head)
+  int nt;          // its tiles per CTA
   int chunk, steps, unit_tok, n_units, grid;
 };
 
@@ -902,17 +924,28 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   s.own_split = own_flat <= 16;
   s.own_tiles = (int)((own_flat + (s.own_split ? 16 : 64) - 1) / (s.own_split ? 16 : 64));
   const int pre_pages = (a.prefix_len + 63) / 64;
-  s.tc = flat > 16;
-  static const int kMinChunk = getenv("PFX_MIN") ? atoi(getenv("PFX_MIN")) : 1;
+  s.pre_tiles = (int)((flat + 15) / 16);
+  // 16-row tiles on mma.sync read the prefix once per tile, but start and end
+  // sooner than the tensor-core kernel: it takes over where an SM would get more
+  // than about 25 tile-pages of 64 dimensions (us, mma.sync / tcgen05: 32 rows x
+  // 512 keys x 8 kv heads of 64 8.0 / 10.1, 64 x 4000 13.7 / 17.1, 128 x 4000
+  // 19.8 / 18.6, 64 x 16000 33.9 / 26.2; 56 x 16000 x 4 of 128 31.3 / 27.2).
+  s.tc = flat > 16 && (long long)s.pre_tiles * c.kv_heads * pre_pages * (c.head_dim / 64) > 25ll * sms;
   if (pre_pages && !s.tc) {
     // Key splits until the CTAs fill the GPU once, at least two pages each.
-    s.sp = (int)std::max(1ll, std::min<long long>(sms / c.kv_heads, (pre_pages + 1) / 2));
+    s.sp = (int)std::max(
+        1ll, std::min<long long>(sms / std::max(1ll, (long long)c.kv_heads * s.pre_tiles), (pre_pages + 1) / 2));
   } else if (pre_pages) {
-    s.steps = (pre_pages + 1) / 2;
-    s.unit_tok = (c.head_dim == 256 ? 1 : 2) * (128 / G);
+    s.steps = pre_pages;
+    // Two tiles per CTA where a CTA has work for a while; one where it has
+    // twelve pages or fewer (64 rows x 4001 keys x 28/4 heads of 128: 25 us
+    // against 28; at 16 pages level; 512 rows x 16384 keys 212 against 178).
+    const long long tiles = (a.rows + 128 / G - 1) / (128 / G);
+    s.nt = c.head_dim == 256 || tiles * c.kv_heads * pre_pages <= 12ll * sms ? 1 : 2;
+    s.unit_tok = s.nt * (128 / G);
     s.n_units = c.kv_heads * ((a.rows + s.unit_tok - 1) / s.unit_tok);
     const long long work = (long long)s.n_units * s.steps;
-    s.chunk = (int)std::max<long long>(kMinChunk, (work + sms - 1) / sms);
+    s.chunk = (int)std::max(1ll, (work + sms - 1) / sms);
     s.grid = (int)((work + s.chunk - 1) / s.chunk);
     // a unit of `steps` touches at most this many runs of `chunk`
     s.sp = (s.steps - 2 + s.chunk) / s.chunk + 1;
@@ -947,6 +980,8 @@ int launch_unit(const CUtensorMap& tk, const CUtensorMap& tv, const PfxParams& p
   if (!configured[dev & 63]) {
     LAYA_CK(cudaFuncSetAttribute(prefix_unit_kernel<E, HD, SPLITK, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  Unit<HD, SPLITK>::SMEM));
+    LAYA_CK(cudaFuncSetAttribute(prefix_unit_kernel<E, HD, SPLITK, OWN>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared));
     configured[dev & 63] = true;
   }
   if (grid > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many attention units");
@@ -955,21 +990,37 @@ int launch_unit(const CUtensorMap& tk, const CUtensorMap& tv, const PfxParams& p
   return 0;
 }
 
+template <typename E, int HD, int NT>
+int launch_tc(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tv_last,
+              const PfxParams& p, int grid, int dev, cudaStream_t st) {
+  using C = Ptc<HD, NT>;
+  static std::atomic<bool> configured[64];
+  if (!configured[dev & 63]) {
+    LAYA_CK(cudaFuncSetAttribute(prefix_tc_kernel<E, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    LAYA_CK(cudaFuncSetAttribute(prefix_tc_kernel<E, HD, NT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared));
+    configured[dev & 63] = true;
+  }
+  LAYA_CK(launch_k(prefix_tc_kernel<E, HD, NT>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, st, false, tq, tk, tv,
+                   tv_last, p));
+  return 0;
+}
+
 template <typename E, int HD>
 int prefix_go(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tv_last, PfxParams p, const Shape& s, int dev, int sms,
               cudaStream_t st) {
   if (s.sp && !s.tc) {
-    p.q_tiles = 1;
-    if (int rc = launch_unit<E, HD, true, false>(tk, tv, p, (long long)p.KV * s.sp, dev, false, st)) return rc;
+    p.q_tiles = s.pre_tiles;
+    if (int rc = launch_unit<E, HD, true, false>(tk, tv, p, (long long)p.KV * s.pre_tiles * s.sp, dev, false, st))
+      return rc;
   } else if (s.sp) {
-    using C = Ptc<HD>;
-    static std::atomic<bool> configured[64];
-    if (!configured[dev & 63]) {
-      LAYA_CK(cudaFuncSetAttribute(prefix_tc_kernel<E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-      configured[dev & 63] = true;
-    }
-    LAYA_CK(launch_k(prefix_tc_kernel<E, HD>, dim3(s.grid), dim3(C::THREADS), (size_t)C::SMEM, st, false, tq, tk, tv,
-                     tv_last, p));
+    int rc;
+    if constexpr (HD == 256)
+      rc = launch_tc<E, HD, 1>(tq, tk, tv, tv_last, p, s.grid, dev, st);
+    else
+      rc = s.nt == 1 ? launch_tc<E, HD, 1>(tq, tk, tv, tv_last, p, s.grid, dev, st)
+                     : launch_tc<E, HD, 2>(tq, tk, tv, tv_last, p, s.grid, dev, st);
+    if (rc) return rc;
   }
   p.q_tiles = s.own_tiles;
   const long long grid = (long long)p.n_seqs * s.own_tiles * p.KV * s.ss;

@@ -297,6 +297,65 @@ def test_attention_batches(n, heads, kv, hd, prefix, dtype):
     b.check(*b.run())
 
 
+# (new rows of each sequence, held tokens, prefix, heads, kv, hd): enough rows and
+# prefix pages for the tensor-core kernel, with one and with two row tiles per
+# CTA, row counts that leave a tile part empty, groups that do not divide 128
+TENSOR_CORE = [
+    ([1] * 60, [3] * 60, 2500, 32, 2, 64),
+    ([5, 0, 40, 1, 3, 17], [5, 9, 200, 1, 64, 100], 4033, 33, 1, 64),
+    ([1] * 61, list(range(1, 62)), 1345, 28, 4, 128),
+    ([1] * 100, [1] * 100, 1250, 8, 2, 256),
+    ([2] * 150, [2] * 150, 2048, 32, 8, 64),
+    ([3] * 50, [70] * 50, 3001, 20, 4, 128),
+    ([7, 0, 90], [7, 0, 90], 5000, 24, 2, 128),
+    ([2] * 120, [5] * 120, 2900, 28, 4, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(TENSOR_CORE)))
+def test_attention_tensor_core_prefix(case, dtype):
+    new, held, prefix, heads, kv, hd = TENSOR_CORE[case]
+    b = Batch(new, held, prefix, heads, kv, hd, dtype, token_major=case % 2 == 1, pad=3 * (case % 3), seed=50 + case)
+    out, lse = b.run()
+    b.check(out, lse)
+    again = b.run()
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("case", [0, 3, 4, 5, 7])
+def test_attention_tensor_core_extremes(case):
+    """Rows whose maximum keeps growing along the keys, and single keys above all."""
+    new, held, prefix, heads, kv, hd = TENSOR_CORE[case]
+    b = Batch(new, held, prefix, heads, kv, hd, F16, seed=70 + case)
+    b.q *= 8
+    b.check(*b.run())
+    # keys that grow along the prefix: O is rescaled again and again
+    grow = torch.linspace(0.02, 4, pages_of(prefix), device="cuda")
+    for i, pg in enumerate(b.prefix_pages.tolist()):
+        b.k[pg] = b.k[pg] * grow[i].to(F16)
+    b.check(*b.run())
+
+
+def test_attention_tensor_core_pages_outside_the_cache():
+    new, held, prefix, heads, kv, hd = TENSOR_CORE[0]
+    b = Batch(new, held, prefix, heads, kv, hd, F16, seed=80, poison=False)
+    pages = b.prefix_pages.clone()
+    b.prefix_pages[3] = -7
+    b.prefix_pages[20:22] = 1 << 29
+    out, lse = b.run()
+    assert status_bits() == 2
+    keep = [i for i in range(pages_of(prefix)) if i not in (3, 20, 21)]
+    want, tol, _, _ = attend_reference(b.q, b.k, b.v, pages[keep], prefix - 3 * 64, b.tables, held, new, b.scale)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+    # none at all: the own keys alone
+    b.prefix_pages.fill_(-1)
+    out, _ = b.run()
+    assert status_bits() == 2
+    want, tol, _, _ = attend_reference(b.q, b.k, b.v, pages, 0, b.tables, held, new, b.scale)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+
+
 def test_attention_long_own_keys_are_split():
     b = Batch([1, 1], [3000, 70], 0, 8, 2, 64, F16, seed=1)
     b.check(*b.run())
@@ -361,7 +420,7 @@ def test_attention_rows_beyond_max_q_and_lengths_beyond_the_table():
 
 
 def test_attention_repeats_bitwise_on_streams_and_in_graphs():
-    a = Batch([1] * 9, list(range(20, 29)), 500, 32, 8, 64, F16, seed=9)
+    a = Batch([1] * 90, list(range(20, 110)), 1500, 32, 8, 64, F16, seed=9)  # tensor-core prefix
     b = Batch([4, 17], [40, 300], 130, 28, 4, 128, F16, seed=10)
     want = [a.run(), b.run()]
     side = [torch.cuda.Stream() for _ in range(2)]
