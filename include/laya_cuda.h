@@ -112,6 +112,16 @@ int laya_decide_batch(laya_model* m, const laya_batch* b, laya_answer* out, int 
  * out_tokens: n_seqs * steps.  stats (may be NULL): [prefill_ms, decode_ms]. */
 int laya_decode(laya_model* m, const int32_t* ids, const int64_t* offsets, int n_seqs, int steps,
                 int32_t* out_tokens, float* stats);
+/* Log probabilities of the sequences' own tokens: row t of a sequence (t = 0 ..
+ * length - 2) is its token t + 1 under the model's distribution after tokens
+ * 0 .. t, computed from full-vocabulary logits by laya_token_logprobs.  A
+ * sequence of `length` tokens gives length - 1 rows; rows are concatenated:
+ * sequence i starts at row offsets[i] - i.  logprobs and entropy (nats; may be
+ * NULL): one float per row; top_ids / top_logprobs: `top` (0..64) likeliest
+ * tokens per row, likeliest first.  Sequences are shared over the model's
+ * devices.  Host buffers.  No counterpart in the reference. */
+int laya_score_tokens(laya_model* m, const int32_t* ids, const int64_t* offsets, int n_seqs, int top, float* logprobs,
+                      float* entropy, int32_t* top_ids, float* top_logprobs);
 void laya_close(laya_model* m);
 /* Thread-local message of the last failure on this thread. */
 const char* laya_last_error(void);

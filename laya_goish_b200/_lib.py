@@ -112,6 +112,7 @@ def lib() -> ctypes.CDLL:
     L.laya_validate.argtypes = [P, ctypes.POINTER(Batch)]
     L.laya_decide_batch.argtypes = [P, ctypes.POINTER(Batch), ctypes.POINTER(Answer), CANCEL_FN, P]
     L.laya_decode.argtypes = [P, P, P, I, I, P, P]
+    L.laya_score_tokens.argtypes = [P, P, P, I, I, P, P, P, P]
     L.laya_close.argtypes = [P]
     L.laya_close.restype = None
     L.laya_dequantize.argtypes = [I, ctypes.c_uint32, P, SZ, P]

@@ -6,6 +6,7 @@
 #include <thread>
 #include <vector>
 
+#include "device_ops.h"
 #include "engine.h"
 #include "gemm.h"
 #include "laya_cuda.h"
@@ -184,6 +185,54 @@ int laya_decode(laya_model* h, const int32_t* ids, const int64_t* offsets, int n
     }
   }
   return 0;
+}
+
+int laya_score_tokens(laya_model* h, const int32_t* ids, const int64_t* offsets, int n_seqs, int top, float* logprobs,
+                      float* entropy, int32_t* top_ids, float* top_logprobs) {
+  return guarded([&]() -> int {
+    if (!h) return fail(LAYA_E_INVALID, "null model");
+    if (n_seqs < 0 || top < 0 || top > LAYA_MAX_TOP) return fail(LAYA_E_INVALID, "invalid score arguments");
+    if (n_seqs == 0) return 0;
+    if (!ids || !offsets || !logprobs || (top && (!top_ids || !top_logprobs)))
+      return fail(LAYA_E_INVALID, "null argument");
+    Model& m = h->m;
+    std::lock_guard<std::mutex> lk(m.mu);
+    if (offsets[0] != 0) return fail(LAYA_E_INVALID, "offsets[0] must be 0");
+    for (int i = 0; i < n_seqs; i++) {
+      if (offsets[i + 1] <= offsets[i]) return fail(LAYA_E_INVALID, "empty token sequence");
+      if (offsets[i + 1] - offsets[i] > m.cfg.ctx)
+        return fail(LAYA_E_INVALID, "token sequence exceeds the context length");
+    }
+    const int64_t total = offsets[n_seqs];
+    for (int64_t t = 0; t < total; t++)
+      if (ids[t] < 0 || ids[t] >= m.cfg.V) return fail(LAYA_E_INVALID, "invalid token sequence");
+    if (top > m.cfg.V) return fail(LAYA_E_INVALID, "more alternatives than the vocabulary holds");
+    const int nd = std::min((int)m.reps.size(), n_seqs);
+    if (nd == 1)
+      return score_shard(m, m.reps[0], ids, offsets, 0, n_seqs, top, logprobs, entropy, top_ids, top_logprobs);
+    // contiguous ranges over the devices, balanced by tokens, one host thread each
+    std::vector<int> cut(nd + 1, n_seqs);
+    cut[0] = 0;
+    int k = 1;
+    for (int i = 0; i < n_seqs && k < nd; i++)
+      if (offsets[i + 1] * nd >= total * k) cut[k++] = i + 1;
+    std::vector<int> rcs(nd, 0);
+    std::vector<std::string> msgs(nd);
+    std::vector<std::thread> th;
+    for (int d = 0; d < nd; d++)
+      th.emplace_back([&, d] {
+        if (cut[d] < cut[d + 1])
+          rcs[d] = guarded([&]() -> int {
+            return score_shard(m, m.reps[d], ids, offsets, cut[d], cut[d + 1], top, logprobs, entropy, top_ids,
+                               top_logprobs);
+          });
+        if (rcs[d]) msgs[d] = g_err;
+      });
+    for (auto& t : th) t.join();
+    for (int d = 0; d < nd; d++)
+      if (rcs[d]) return fail(rcs[d], msgs[d]);
+    return 0;
+  });
 }
 
 void laya_close(laya_model* h) {

@@ -1373,4 +1373,108 @@ int decide_shard(Model& m, Replica& r, const laya_batch& b, int r0, int r1, laya
   return 0;
 }
 
+// ---------------------------------------------------------------- score
+
+// Log probabilities of sequences [s0, s1)'s own tokens: full-vocabulary logits
+// of every position but the last (waves of at most wave_tokens() prompt tokens,
+// logits in chunks of 256 MB), read by token_logprobs.  The outputs are the
+// whole call's, indexed by the sequence's first row.
+int score_shard(Model& m, Replica& r, const int32_t* ids, const int64_t* off, int s0, int s1, int top, float* logprobs,
+                float* entropy, int32_t* top_ids, float* top_logprobs) {
+  const Config& c = m.cfg;
+  LAYA_CK(cudaSetDevice(r.device));
+  int rc;
+  if ((rc = timing_begin_call(r)) || (rc = ensure_head16(m, r))) return rc;
+  LAYA_CK(cudaMemsetAsync(r.err, 0, 4, r.stream));
+  DevBuf dtok, dout;
+  struct Release {
+    DevBuf *a, *b;
+    cudaStream_t st;
+    ~Release() {
+      cudaStreamSynchronize(st);  // an error return may leave work that uses them
+      a->release();
+      b->release();
+    }
+  } guard{&dtok, &dout, r.stream};
+  const long budget = wave_tokens();
+  for (int i = s0; i < s1;) {
+    long tok = 0;
+    int j = i;
+    while (j < s1 && (j == i || tok + (off[j + 1] - off[j]) <= budget)) {
+      tok += off[j + 1] - off[j];
+      j++;
+    }
+    PassPlan p;
+    std::vector<int> tables, next;
+    int pages = 0;
+    for (int q = i; q < j; q++) {
+      const int len = (int)(off[q + 1] - off[q]), toff = (int)tables.size(), row0 = (int)p.ids.size();
+      for (int pg = 0; pg < (len + PAGE - 1) / PAGE; pg++) tables.push_back(pages++);
+      for (int t = 0; t < len; t++) {
+        p.ids.push_back(ids[off[q] + t]);
+        p.pos.push_back(t);
+        p.slot.push_back(tables[toff + t / PAGE] * PAGE + t % PAGE);
+        if (t + 1 < len) {
+          p.read_rows.push_back(row0 + t);
+          next.push_back(ids[off[q] + t + 1]);
+        }
+      }
+      for (int t0 = 0; t0 < len; t0 += kAttnRows)
+        p.items.push_back({row0 + t0, std::min(kAttnRows, len - t0), t0, toff});
+    }
+    const int R = (int)next.size();
+    if (R) {
+      if ((rc = ensure_kv(m, r, pages)) || (rc = r.hid32.ensure((size_t)R * c.d * 4)) ||
+          (rc = r.hid16.ensure((size_t)R * c.d * 2)))
+        return rc;
+      r.arm_start = true;
+      if ((rc = run_forward(m, r, p, tables, 0, nullptr, nullptr, nullptr))) return rc;
+      // per row: log probability, entropy, then the alternatives' log probabilities and ids
+      const size_t width = 2 + 2 * (size_t)top;
+      if ((rc = dtok.ensure((size_t)R * 4)) || (rc = dout.ensure(R * width * 4))) return rc;
+      LAYA_CK(cudaMemcpyAsync(dtok.p, next.data(), (size_t)R * 4, cudaMemcpyHostToDevice, r.stream));
+      r.h2d += (long long)R * 4;
+      float *lp = dout.as<float>(), *ent = lp + R, *tlp = ent + R;
+      int32_t* tid = reinterpret_cast<int32_t*>(tlp + (size_t)R * top);
+      const int chunk = std::max(128, (int)((256ull << 20) / ((size_t)c.V * 4)) / 128 * 128);
+      if ((rc = r.flog.ensure((size_t)std::min(chunk, R) * c.V * 4))) return rc;
+      for (int q0 = 0; q0 < R; q0 += chunk) {
+        const int mr = std::min(chunk, R - q0);
+        GemmArgs a{};
+        a.M = mr;
+        a.N = c.V;
+        a.K = c.d;
+        a.out = r.flog.p;
+        a.ldo = c.V;
+        if ((rc = gemm(r, P_GEMM_HEAD, EPI_F32, r.hid16.as<half>() + (size_t)q0 * c.d, c.d, r.head16, c.d, a)))
+          return rc;
+        r.launches++;
+        if ((rc = laya_token_logprobs(LAYA_TYPE_F32, r.flog.p, c.V, mr, c.V, dtok.as<int32_t>() + q0, 1, 1, top,
+                                      lp + q0, ent + q0, nullptr, top ? tid + (size_t)q0 * top : nullptr,
+                                      top ? tlp + (size_t)q0 * top : nullptr, r.stream)))
+          return rc;
+      }
+      if ((rc = timing_mark_end(r))) return rc;
+      const size_t first = (size_t)off[i] - i;  // rows of the sequences before
+      LAYA_CK(cudaMemcpyAsync(logprobs + first, lp, (size_t)R * 4, cudaMemcpyDeviceToHost, r.stream));
+      if (entropy) LAYA_CK(cudaMemcpyAsync(entropy + first, ent, (size_t)R * 4, cudaMemcpyDeviceToHost, r.stream));
+      if (top) {
+        LAYA_CK(cudaMemcpyAsync(top_logprobs + first * top, tlp, (size_t)R * top * 4, cudaMemcpyDeviceToHost, r.stream));
+        LAYA_CK(cudaMemcpyAsync(top_ids + first * top, tid, (size_t)R * top * 4, cudaMemcpyDeviceToHost, r.stream));
+      }
+      r.d2h += (long long)(R * width * 4) + 4;
+      LAYA_CK(cudaStreamSynchronize(r.stream));
+      unsigned err = 0;
+      LAYA_CK(cudaMemcpy(&err, r.err, 4, cudaMemcpyDeviceToHost));
+      if (err)
+        return fail(LAYA_E_TIMEOUT, "a device-side wait ran out of its budget (code " + std::to_string(err) + ")");
+      if (r.prof) prof_collect(r);
+      for (int q = 0; q < R; q++)
+        if (!std::isfinite(logprobs[first + q])) return fail(LAYA_E_NONFINITE, "non-finite model output");
+    }
+    i = j;
+  }
+  return 0;
+}
+
 }  // namespace laya

@@ -182,6 +182,8 @@ Q8Weights q8_down(const Config& c, const Layer& L);
 Q8Weights q8_head(const Replica& r);
 int decide_shard(Model& m, Replica& r, const laya_batch& b, int r0, int r1, laya_answer* out,
                  int (*canceled)(void*), void* user, std::mutex* cancel_mu);
+int score_shard(Model& m, Replica& r, const int32_t* ids, const int64_t* off, int s0, int s1, int top, float* logprobs,
+                float* entropy, int32_t* top_ids, float* top_logprobs);
 int validate_batch(const Config& c, const laya_batch* b);
 int decode_run(Model& m, Replica& r, const int32_t* ids, const int64_t* off, int n_seqs, int steps, int32_t* out,
                float* stats);

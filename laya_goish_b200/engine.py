@@ -7,6 +7,8 @@ engine's plugin boundary:
 * ``Engine.decide(...)``          — Backend::decide for one request (src/models/mod.rs:16-22)
 * ``Engine.decide_batch(...)``    — /v1/decide/batch: many requests sharing the questions
                                      (src/server.rs:235-332), sharded across GPUs
+* ``Engine.score_tokens(...)``    — log probabilities, entropy and alternatives of a prompt's own tokens
+                                     (no counterpart in the reference)
 * ``dequantize`` / ``matrix_apply`` — gguf::decode (src/gguf.rs:250-336) and
                                      Matrix::apply (src/tensor.rs:10-39)
 
@@ -147,6 +149,23 @@ class Engine:
                                      args.offsets.ctypes.data_as(ctypes.c_void_p), len(contexts), steps,
                                      out.ctypes.data_as(ctypes.c_void_p), stats.ctypes.data_as(ctypes.c_void_p)))
         return out, {"prefill_ms": float(stats[0]), "decode_ms": float(stats[1])}
+
+    def score_tokens(self, prompts, top: int = 0) -> list[dict]:
+        """Log probabilities of each prompt's own tokens given those before them:
+        per prompt of n tokens {"logprobs": [n - 1], "entropy": [n - 1] (nats),
+        "top_ids": [n - 1, top], "top_logprobs": [n - 1, top]}, row t for token
+        t + 1; the likeliest alternative first."""
+        args = _BatchArgs(prompts, [])
+        first = args.offsets - np.arange(len(args.offsets))
+        rows = max(0, int(first[-1]))
+        lp, ent = np.zeros(rows, np.float32), np.zeros(rows, np.float32)
+        ids, tlp = np.zeros((rows, max(top, 0)), np.int32), np.zeros((rows, max(top, 0)), np.float32)
+        check(_lib.lib().laya_score_tokens(self._h, args.ids.ctypes.data_as(ctypes.c_void_p),
+                                           args.offsets.ctypes.data_as(ctypes.c_void_p), len(prompts), top,
+                                           lp.ctypes.data_as(ctypes.c_void_p), ent.ctypes.data_as(ctypes.c_void_p),
+                                           ids.ctypes.data_as(ctypes.c_void_p), tlp.ctypes.data_as(ctypes.c_void_p)))
+        return [{"logprobs": lp[a:b], "entropy": ent[a:b], "top_ids": ids[a:b], "top_logprobs": tlp[a:b]}
+                for a, b in zip(first[:-1], first[1:])]
 
     def forward(self, ids, read) -> np.ndarray:
         ids = np.ascontiguousarray(np.asarray(ids, np.int32))

@@ -130,6 +130,11 @@ def test_token_logprobs_arguments():
     invalid(L.laya_device_status(0, None), "null")
 
 
+def test_score_arguments():
+    L = _lib.lib()
+    invalid(L.laya_score_tokens(None, A, A, 1, 0, A, None, None, None), "null model")
+
+
 def test_host_tensors_are_refused():
     from laya_goish_b200 import device
 
