@@ -322,9 +322,9 @@ int laya_kv_append(const laya_kv_pages* cache, uint32_t type, const void* k, con
  * kv_heads); rows that see no key give 0 and lse -inf.  Rows of no sequence
  * are left as they were.  Scores, softmax statistics and sums are 32-bit;
  * probabilities are rounded to the cache's type for the second product.
- * Keys of a page outside the cache count as unseen.  Values that no row may
- * see (past a length) may be anything, NaN included; what a sequence holds
- * within its length has to be finite. */
+ * Keys of a page outside the cache count as unseen.  What a row does not see
+ * (past a length, later tokens of its sequence) is not in its result, whatever
+ * its value, NaN included; an infinity that it sees gives that or NaN. */
 typedef struct laya_prefix_args {
   const void* q;                /* rows x heads x head_dim, the cache's type, row stride q_stride elements */
   int64_t q_stride;             /* a multiple of 8; q 16-byte aligned */
@@ -357,7 +357,8 @@ int laya_prefix_attention(const laya_kv_pages* cache, const laya_prefix_args* a,
  *   ascending id: top_ids / top_logprobs [rows][top].
  * A logit of -inf is a token that is not there: it is no alternative (id -1,
  * -inf where fewer than `top` are there), and a row of them alone has lse and
- * logprobs -inf and entropy 0.  A row with NaN or +inf gives NaN, ids -1. */
+ * logprobs -inf and entropy 0.  A row with NaN or +inf gives NaN, ids -1;
+ * so may one with a logit above 2e38. */
 #define LAYA_MAX_TOP 64
 int laya_token_logprobs(uint32_t type, const void* logits, int64_t row_stride, int rows, int vocab,
                         const int32_t* tokens, int64_t token_stride, int n_tokens, int top, float* logprobs,

@@ -15,11 +15,12 @@
 // are not split, the own-keys kernel writes the output itself.  (Joining in
 // the own-keys kernel, behind its pages, was slower: its few rows per CTA
 // expose the latency of every plane's load.  512 rows x 16384 keys x 32 heads
-// of 128: 280 us against 230.)
+// of 128, with the prefix kernel of that time: 280 us against 230; now 180.)
 #include <cuda.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "device_ops.h"
 #include "gemm.h"
@@ -69,6 +70,7 @@ struct Mma<half> {
     mma16816(d, a, b0, b1);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_h2(a, b); }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<half2*>(&x)); }
 };
 template <>
 struct Mma<__nv_bfloat16> {
@@ -82,12 +84,24 @@ struct Mma<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) {
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  }
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// log2 of a sum l of 2^(x - m2); -inf of an empty one, a NaN stays.
+__device__ __forceinline__ float log2_sum(float m2, float l) { return l == 0.f ? -INFINITY : m2 + log2f(l); }
+
+// Bits 15 and 31: the halves of two packed 16-bit values that are infinite or NaN.
+template <typename E>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  return ((x & 0x7fff7fffu) + (__is_same(E, half) ? 0x04000400u : 0x00800080u)) & 0x80008000u;
 }
 
 // Byte offset of 16-byte piece c of row r in a [HD / 64 blocks][R rows][128 B]
@@ -163,7 +177,10 @@ struct Unit {
 // over all rows of the batch.
 // A unit is short (a few pages), so its chain of latencies (sizes, page
 // numbers, pages, partials, output) is hidden by other units: small rings,
-// two or three CTAs per SM (measured in DESIGN's table).
+// two or three CTAs per SM (us, against rings that fill an SM's shared memory
+// and one CTA: 64 sequences of one row 25 / 31, 33 to 96 rows each 26 / 33, 512
+// single rows behind 16384 shared keys 180 / 243, where they also find room
+// beside the prefix kernel).
 template <typename E, int HD, bool SPLITK, bool OWN>
 __global__ void __maxnreg__((HD == 256 ? 255 : 168))
     prefix_unit_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -268,118 +285,170 @@ __global__ void __maxnreg__((HD == 256 ? 255 : 168))
       }
     }
   };
+  int filled = -1;  // the last page that this (leading) warp asked for
   if (leads)
-    for (int i = first; i < min(np, C::S); i += STEP) fill(i);
-  {
-    // visible keys of this thread's two rows
-    int vis[2];
+    for (int i = first; i < min(np, C::S); i += STEP) fill(filled = i);
+  bool live = true;  // false once a wait ran out; the warps keep to the same barriers
+  // visible keys of this thread's two rows
+  int vis[2];
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-      vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
-    constexpr int KEYS = C::KEYS;
-    const int koff = SPLITK ? (warp & 1) * 32 : 0;  // this warp's first key of a page
-    for (int i = first; i < np; i += STEP) {
-      const int st = i % C::S;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (i / C::S) & 1, kBudget))) {
-        if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
-        // give the copies that are still on their way as long again
-        for (int x = i; x < min(np, i + C::S); x += STEP) mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget);
-        break;
-      }
-      const uint8_t* sK = sm + st * C::STAGE;
-      uint8_t* sV = sm + st * C::STAGE + C::PAGE;
-      const int key0 = (p0 + i) * 64;
-      if (page_ok[st]) {
-        if (key0 + 64 > sq.keys) {
-          // Rows past the last key may hold anything, and 0 * NaN is NaN: zero them.
-          const int from = max(sq.keys - key0, koff);
-          for (int x = (SPLITK ? lane : tid); x < (koff + KEYS - from) * (HD / 8); x += SPLITK ? 32 : 128)
-            *reinterpret_cast<uint4*>(sV + tile_off<64>(from + x / (HD / 8), x % (HD / 8))) =
-                make_uint4(0u, 0u, 0u, 0u);
-          if (SPLITK)
-            __syncwarp();
-          else
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-        }
-        float sc[KEYS / 8][4];
-#pragma unroll
-        for (int j = 0; j < KEYS / 8; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-        const int mat = lane / 8;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; kk++) {
-          uint32_t qa[4];
-          ldsm_x4(qa, sQ + tile_off<ROWS>(wr + (lane % 8) + (mat % 2) * 8, kk * 2 + mat / 2));
-#pragma unroll
-          for (int nj = 0; nj < KEYS / 8; nj += 2) {
-            uint32_t bf[4];
-            ldsm_x4(bf, sK + tile_off<64>(koff + nj * 8 + (lane % 8) + (mat / 2) * 8, kk * 2 + (mat % 2)));
-            Mma<E>::run(sc[nj], qa, bf[0], bf[1]);
-            Mma<E>::run(sc[nj + 1], qa, bf[2], bf[3]);
-          }
-        }
-        if (key0 + 64 > min(first_vis, sq.keys)) {
-#pragma unroll
-          for (int j = 0; j < KEYS / 8; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (key0 + koff + j * 8 + 2 * t + (e & 1) >= vis[e >> 1]) sc[j][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < KEYS / 8; j++) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[h], mx);
-          // a row that has seen no key yet keeps reference 0: its terms are 2^-inf = 0
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          const float corr = ex2((m[h] - ref) * p.scale_log2), off = -ref * p.scale_log2;
-          m[h] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < KEYS / 8; j++) {
-            sc[j][2 * h] = ex2(fmaf(sc[j][2 * h], p.scale_log2, off));
-            sc[j][2 * h + 1] = ex2(fmaf(sc[j][2 * h + 1], p.scale_log2, off));
-            sum += sc[j][2 * h] + sc[j][2 * h + 1];
-          }
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          l[h] = l[h] * corr + sum;
-#pragma unroll
-          for (int d = 0; d < HD / 8; d++) {
-            acc[d][2 * h] *= corr;
-            acc[d][2 * h + 1] *= corr;
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < KEYS / 16; kk++) {
-          // probabilities rounded to the cache's type: the second product's operand
-          const uint32_t pa[4] = {Mma<E>::pack(sc[2 * kk][0], sc[2 * kk][1]), Mma<E>::pack(sc[2 * kk][2], sc[2 * kk][3]),
-                                  Mma<E>::pack(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
-                                  Mma<E>::pack(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
-#pragma unroll
-          for (int nd = 0; nd < HD / 8; nd += 2) {
-            uint32_t bf[4];
-            ldsm_x4_t(bf, sV + tile_off<64>(koff + kk * 16 + (lane % 8) + (mat % 2) * 8, nd + mat / 2));
-            Mma<E>::run(acc[nd], pa, bf[0], bf[1]);
-            Mma<E>::run(acc[nd + 1], pa, bf[2], bf[3]);
-          }
-        }
-      }
+  for (int h = 0; h < 2; h++)
+    vis[h] = OWN ? min(sq.keys, sq.len - sq.nq + (f0 + wr + g + 8 * h) / p.G + 1) : p.prefix_len;
+  constexpr int KEYS = C::KEYS;
+  const int koff = SPLITK ? (warp & 1) * 32 : 0;  // this warp's first key of a page
+  const int me = SPLITK ? lane : tid, sharers = SPLITK ? 32 : 128;  // threads that share those keys
+  auto sync = [&] {
+    if (SPLITK)
       __syncwarp();
-      if (i + C::S < np) {  // the stage's next page, once its warps have left it
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (leads) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], (i / C::S) & 1, kBudget))) {
-            if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
-            break;
+    else
+      __syncthreads();
+  };
+  for (int i = first; i < np; i += STEP) {
+    const int st = i % C::S;
+    if (live && !__all_sync(0xffffffffu, mbar_wait(&full[st], (i / C::S) & 1, kBudget))) {
+      live = false;
+      if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
+    }
+    const uint8_t* sK = sm + st * C::STAGE;
+    uint8_t* sV = sm + st * C::STAGE + C::PAGE;
+    const int key0 = (p0 + i) * 64;
+    const bool ok = live && page_ok[st];
+    float sc[KEYS / 8][4];
+    if (ok) {
+#pragma unroll
+      for (int j = 0; j < KEYS / 8; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      const int mat = lane / 8;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; kk++) {
+        uint32_t qa[4];
+        ldsm_x4(qa, sQ + tile_off<ROWS>(wr + (lane % 8) + (mat % 2) * 8, kk * 2 + mat / 2));
+#pragma unroll
+        for (int nj = 0; nj < KEYS / 8; nj += 2) {
+          uint32_t bf[4];
+          ldsm_x4(bf, sK + tile_off<64>(koff + nj * 8 + (lane % 8) + (mat / 2) * 8, kk * 2 + (mat % 2)));
+          Mma<E>::run(sc[nj], qa, bf[0], bf[1]);
+          Mma<E>::run(sc[nj + 1], qa, bf[2], bf[3]);
+        }
+      }
+      if (key0 + 64 > min(first_vis, sq.keys)) {
+#pragma unroll
+        for (int j = 0; j < KEYS / 8; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (key0 + koff + j * 8 + 2 * t + (e & 1) >= vis[e >> 1]) sc[j][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KEYS / 8; j++) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[h], mx);
+        // a row that has seen no key yet keeps reference 0: its terms are 2^-inf = 0
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2((m[h] - ref) * p.scale_log2), off = -ref * p.scale_log2;
+        m[h] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KEYS / 8; j++) {
+          sc[j][2 * h] = ex2(fmaf(sc[j][2 * h], p.scale_log2, off));
+          sc[j][2 * h + 1] = ex2(fmaf(sc[j][2 * h + 1], p.scale_log2, off));
+          sum += sc[j][2 * h] + sc[j][2 * h + 1];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        l[h] = l[h] * corr + sum;
+#pragma unroll
+        for (int d = 0; d < HD / 8; d++) {
+          acc[d][2 * h] *= corr;
+          acc[d][2 * h + 1] *= corr;
+        }
+      }
+    }
+    // A probability of 0 times NaN or infinity is NaN.  Keys that no row of the
+    // tile sees may hold anything: their values become 0.
+    const bool tail = key0 + 64 > last_vis;
+    if (tail && ok) {
+      const int from = max(last_vis - key0, koff);
+      for (int x = me; x < (koff + KEYS - from) * (HD / 8); x += sharers)
+        *reinterpret_cast<uint4*>(sV + tile_off<64>(from + x / (HD / 8), x % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    // Keys that some of its rows see and some do not (later tokens of the
+    // sequence): what is not finite is added to the rows that see it by hand
+    // (any probability times it is itself) and leaves the page.
+    const int lo = max(first_vis - key0, koff), hi = min(last_vis - key0, koff + KEYS);
+    if (OWN && lo < hi) {
+      bool odd = false;
+      if (ok)
+        for (int x = me; x < (hi - lo) * (HD / 8); x += sharers) {
+          const uint4 w = *reinterpret_cast<const uint4*>(sV + tile_off<64>(lo + x / (HD / 8), x % (HD / 8)));
+          odd |= (not_finite<E>(w.x) | not_finite<E>(w.y) | not_finite<E>(w.z) | not_finite<E>(w.w)) != 0;
+        }
+      if (SPLITK ? __any_sync(0xffffffffu, odd) : __syncthreads_or(odd)) {
+        if (ok)
+#pragma unroll 1
+          for (int key = lo; key < hi; key++)
+#pragma unroll
+            for (int d = 0; d < HD / 8; d++) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(sV + tile_off<64>(key, d) + 4 * t);
+              const uint32_t bad = not_finite<E>(w);
+              const float2 v = Mma<E>::unpack(w);
+#pragma unroll
+              for (int h = 0; h < 2; h++)
+                if (key0 + key < vis[h]) {
+                  if (bad & 0x8000u) acc[d][2 * h] += v.x;
+                  if (bad & 0x80000000u) acc[d][2 * h + 1] += v.y;
+                }
+            }
+        sync();
+        if (ok)
+#pragma unroll 1
+          for (int x = me; x < (hi - lo) * (HD / 2); x += sharers) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(sV + tile_off<64>(lo + x / (HD / 2), x % (HD / 2) / 4) + x % 4 * 4);
+            const uint32_t bad = not_finite<E>(*w);
+            *w &= ~((bad & 0x8000u ? 0xffffu : 0u) | (bad & 0x80000000u ? 0xffff0000u : 0u));
           }
-          fill(i + C::S);
+        sync();
+      } else if (SPLITK) {
+        __syncwarp();
+      }
+    } else if (tail) {
+      sync();
+    }
+    if (ok) {
+      const int mat = lane / 8;
+#pragma unroll
+      for (int kk = 0; kk < KEYS / 16; kk++) {
+        // probabilities rounded to the cache's type: the second product's operand
+        const uint32_t pa[4] = {Mma<E>::pack(sc[2 * kk][0], sc[2 * kk][1]), Mma<E>::pack(sc[2 * kk][2], sc[2 * kk][3]),
+                                Mma<E>::pack(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
+                                Mma<E>::pack(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
+#pragma unroll
+        for (int nd = 0; nd < HD / 8; nd += 2) {
+          uint32_t bf[4];
+          ldsm_x4_t(bf, sV + tile_off<64>(koff + kk * 16 + (lane % 8) + (mat % 2) * 8, nd + mat / 2));
+          Mma<E>::run(acc[nd], pa, bf[0], bf[1]);
+          Mma<E>::run(acc[nd + 1], pa, bf[2], bf[3]);
+        }
+      }
+    }
+    __syncwarp();
+    if (live && i + C::S < np) {  // the stage's next page, once its warps have left it
+      if (lane == 0) mbar_arrive(&empty[st]);
+      if (leads) {
+        if (__all_sync(0xffffffffu, mbar_wait(&empty[st], (i / C::S) & 1, kBudget))) {
+          fill(filled = i + C::S);
+        } else {
+          live = false;
+          if (lane == 0) atomicOr(p.status, LAYA_STATUS_TIMEOUT);
         }
       }
     }
   }
+  // after a timeout: the copies that are still on their way land before the ring is used again
+  if (!live && leads)
+    for (int x = filled; x >= 0 && x > filled - C::S; x -= STEP) mbar_wait(&full[x % C::S], (x / C::S) & 1, kBudget);
   // ---- the tile's results
   if constexpr (SPLITK) {
     // join the warps' states through the (drained) ring: [NW][16][HD + 2]
@@ -418,7 +487,7 @@ __global__ void __maxnreg__((HD == 256 ? 255 : 168))
         v1 = fmaf(wt, x.y, v1);
       }
       const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-      const float l2 = M == -INFINITY ? -INFINITY : M + log2f(sum);
+      const float l2 = log2_sum(M, sum);
       if (partial) {
         if (d == 0) p.part_l[plane * rowsH + th] = l2;
         *reinterpret_cast<float2*>(p.part_o + (plane * rowsH + th) * HD + d) = make_float2(v0 * inv, v1 * inv);
@@ -437,7 +506,7 @@ __global__ void __maxnreg__((HD == 256 ? 255 : 168))
         const int f = f0 + r, tok = sq.q0 + f / p.G, h = kvh * p.G + f % p.G;
         const size_t th = (size_t)tok * p.H + h;
         const float inv = l[hh] > 0.f || l[hh] != l[hh] ? 1.f / l[hh] : 0.f;
-        const float l2 = m[hh] == -INFINITY ? -INFINITY : m[hh] * p.scale_log2 + log2f(l[hh]);
+        const float l2 = log2_sum(m[hh] * p.scale_log2, l[hh]);
         if (partial) {
           if (t == 0) p.part_l[plane * rowsH + th] = l2;
 #pragma unroll
@@ -799,7 +868,7 @@ __global__ void __maxnreg__(kTcRegs)
       if (busy) {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const size_t th = (size_t)tok * p.H + h, rowsH = (size_t)p.rows * p.H;
-        if (valid) p.part_l[r.plane * rowsH + th] = mref == -INFINITY ? -INFINITY : mref - log2f(inv);
+        if (valid) p.part_l[r.plane * rowsH + th] = log2_sum(mref, l);
         // A lane holds a row; through shared memory two lanes write 32 bytes of one
         // (16-byte pieces, piece j of row i at j ^ (i / 4 % 2)).
         uint4* stage = reinterpret_cast<uint4*>(sm + C::OFF_OUT) + (warp - 4) * 64;
@@ -899,7 +968,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PfxParams p, int
     }
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  if (p.lse && sub == 0) p.lse[th] = M == -INFINITY ? -INFINITY : (M + log2f(sum)) * kLn2;
+  if (p.lse && sub == 0) p.lse[th] = log2_sum(M, sum) * kLn2;
   *reinterpret_cast<uint4*>(static_cast<E*>(p.out) + (long long)tok * p.out_stride + h * HD + sub * 8) =
       make_uint4(Mma<E>::pack(acc[0] * inv, acc[1] * inv), Mma<E>::pack(acc[2] * inv, acc[3] * inv),
                  Mma<E>::pack(acc[4] * inv, acc[5] * inv), Mma<E>::pack(acc[6] * inv, acc[7] * inv));
@@ -1067,7 +1136,8 @@ extern "C" size_t laya_prefix_attention_workspace(const laya_kv_pages* cache, co
 extern "C" int laya_prefix_attention(const laya_kv_pages* cache, const laya_prefix_args* a, void* stream) {
   return guarded([&]() -> int {
     if (int rc = check_sizes(cache, a)) return rc;
-    if (!(a->scale > 0.f) || a->scale > 3e38f) return fail(LAYA_E_INVALID, "scale must be positive and finite");
+    if (!(a->scale > 0.f) || !std::isfinite(a->scale * 1.4426950408889634f))
+      return fail(LAYA_E_INVALID, "scale must be positive and finite");
     if (a->rows == 0 || a->n_seqs == 0 || a->max_q == 0) return 0;
     if (!cache->k || !cache->v || !a->q || !a->out || !a->offsets || !a->lens || (a->prefix_len && !a->prefix_pages) ||
         (a->width && !a->tables))

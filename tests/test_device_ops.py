@@ -130,6 +130,12 @@ def test_token_logprobs_arguments():
     invalid(L.laya_device_status(0, None), "null")
 
 
+def test_prefix_attention_scale_stays_finite_in_log2_units():
+    a = _lib.PrefixArgs(q=A, q_stride=2048, rows=3, heads=32, offsets=A, n_seqs=2, max_q=2, prefix_pages=A,
+                        prefix_len=100, width=2, tables=A, table_stride=2, lens=A, scale=2.5e38, out=A, out_stride=2048)
+    invalid(_lib.lib().laya_prefix_attention(ctypes.byref(cache()), ctypes.byref(a), None), "scale")
+
+
 def test_score_arguments():
     L = _lib.lib()
     invalid(L.laya_score_tokens(None, A, A, 1, 0, A, None, None, None), "null model")

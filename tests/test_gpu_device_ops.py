@@ -715,3 +715,74 @@ def test_refusals():
     with pytest.raises(LayaError, match="empty vocabulary"):
         device.token_logprobs(x[:, :0], i32([[0], [0]]))
     device.check_status()
+
+
+# What a row may not see is not in its result, whatever its value: later tokens
+# of its own sequence with NaN or infinite K and V, in both forms of the own-keys
+# kernel (few rows per kv head, many), with and without a prefix.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("nq,own,heads,kv,prefix", [(5, 9, 4, 2, 0), (5, 67, 4, 2, 100), (40, 40, 4, 1, 0),
+                                                    (150, 170, 2, 2, 70), (16, 200, 8, 8, 0)])
+def test_later_tokens_may_hold_anything(dtype, hd, nq, own, heads, kv, prefix):
+    gen = torch.Generator().manual_seed(nq * own + hd)
+    pages, width, pre = 12, (own + 63) // 64, (prefix + 63) // 64
+    k = torch.randn(pages, kv, 64, hd, generator=gen).to(dtype).cuda()
+    v = torch.randn(pages, kv, 64, hd, generator=gen).to(dtype).cuda()
+    q = torch.randn(nq, heads, hd, generator=gen).to(dtype).cuda()
+    order = torch.randperm(pages, generator=gen).to(torch.int32).cuda()
+    prefix_pages, tables = order[:pre], order[pre:pre + width].reshape(1, width).contiguous()
+    lens, offsets = torch.tensor([own], dtype=torch.int32).cuda(), torch.tensor([0, nq], dtype=torch.int32).cuda()
+
+    def run():
+        lse = torch.empty(nq, heads, dtype=torch.float32, device="cuda")
+        return device.prefix_attention(q, device.KVPages(k, v), prefix_pages, prefix, tables, lens, offsets, nq,
+                                       lse=lse), lse
+
+    def place(tok):
+        return int(tables[0, tok // 64]), tok % 64
+
+    clean, clean_lse = run()
+    for back, bad in ((1, float("nan")), (2, float("inf")), (nq // 2, float("-inf"))):
+        first = nq - back  # the first row that sees the bad token
+        page, at = place(own - back)
+        saved = k[page, :, at].clone(), v[page, :, at].clone()
+        v[page, :, at, ::3] = bad
+        out, lse = run()
+        assert torch.equal(out[:first], clean[:first]) and torch.equal(lse, clean_lse)
+        seen = out[first:, :, ::3].float()
+        # (an infinity times a probability that the type rounds to 0 is NaN)
+        assert (seen.isnan() | (seen == bad)).all()
+        assert torch.equal(out[first:, :, 1::3], clean[first:, :, 1::3])
+        k[page, :, at] = bad
+        out, lse = run()
+        assert torch.equal(out[:first], clean[:first]) and torch.equal(lse[:first], clean_lse[:first])
+        k[page, :, at], v[page, :, at] = saved
+    device.check_status()
+
+
+@pytest.mark.parametrize("rows,prefix", [(1, 70), (40, 200), (400, 3000)])
+def test_a_query_that_is_not_a_number(rows, prefix):
+    """NaN queries give NaN and leave the other rows alone (prefix kernels and join)."""
+    gen = torch.Generator().manual_seed(rows)
+    pages = (prefix + 63) // 64 + 1
+    k = torch.randn(pages, 2, 64, 128, generator=gen).half().cuda()
+    v = torch.randn(pages, 2, 64, 128, generator=gen).half().cuda()
+    q = torch.randn(rows, 4, 128, generator=gen).half().cuda()
+    order = torch.arange(pages, dtype=torch.int32).cuda()
+    tables = torch.full((rows, 1), pages - 1, dtype=torch.int32).cuda()
+    lens = torch.full((rows,), 3, dtype=torch.int32).cuda()
+    offsets = torch.arange(rows + 1, dtype=torch.int32).cuda()
+    res = []
+    for i in range(2):
+        if i:
+            q[rows // 2, 1] = float("nan")
+        lse = torch.empty(rows, 4, dtype=torch.float32, device="cuda")
+        out = device.prefix_attention(q, device.KVPages(k, v), order[:-1], prefix, tables, lens, offsets, 1, lse=lse)
+        res.append((out, lse))
+    device.check_status()
+    (a, al), (b, bl) = res
+    hit = torch.zeros(rows, 4, dtype=torch.bool, device="cuda")
+    hit[rows // 2, 1] = True
+    assert b[hit].isnan().all() and bl[hit].isnan().all()
+    assert torch.equal(a[~hit], b[~hit]) and torch.equal(al[~hit], bl[~hit])
