@@ -786,3 +786,15 @@ def test_a_query_that_is_not_a_number(rows, prefix):
     hit[rows // 2, 1] = True
     assert b[hit].isnan().all() and bl[hit].isnan().all()
     assert torch.equal(a[~hit], b[~hit]) and torch.equal(al[~hit], bl[~hit])
+
+
+# Few rows over a long prefix: many partial results per row, which the join
+# shares out (both prefix kernels, a count that leaves the last group idle).
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,prefix,heads,kv,hd", [([1], 2500, 4, 1, 64), ([1, 1, 1], 7000, 10, 2, 128),
+                                                    ([2, 0, 1], 2177, 4, 2, 256), ([1] * 33, 6000, 8, 2, 256),
+                                                    ([20], 6400, 7, 1, 64), ([1] * 5, 16000, 16, 1, 128)])
+def test_attention_many_partial_results(new, prefix, heads, kv, hd, dtype):
+    held = [n + 40 * (i % 3) for i, n in enumerate(new)]
+    b = Batch(new, held, prefix, heads, kv, hd, dtype, pad=2, seed=prefix)
+    b.check(*b.run())
