@@ -538,7 +538,8 @@ __global__ void __maxnreg__((HD == 256 ? 255 : 168))
 //   S = Q K^T   (M 128, N 64, into one of the tile's two score buffers in TMEM),
 //   P = 2^(S - ref),  O += P V
 // with P written back over S in TMEM as the next product's A operand.
-//   warp 0        TMA: Q, then K and V of each page into one ring of stages
+//   warp 0        TMA: Q, then K and V of each page into one ring of stages, in
+//                 the order of the products
 //   warp 1        one thread issues the products, the scores two pages ahead:
 //                 the softmax of a page does not wait for its scores
 //   warps 4 ..    softmax, four warps per tile, thread = row = TMEM lane.  O is
@@ -676,25 +677,33 @@ __global__ void __maxnreg__(kTcRegs)
             for (int hb = 0; hb < HD / 64; hb++)
               tma_load_3d(sm + t * C::Q_TILE + hb * 16384, &tq, q_full, hb * 64, r.kvh * G, r.tok0 + t * TT);
           k++;
-          int next = p.prefix_pages[r.s0];
-          for (int s = r.s0; s < r.s1 && live; s++) {
-            int page = next;
-            if (s + 1 < r.s1) next = p.prefix_pages[s + 1];
-            if (page < 0 || page >= p.pages) {
-              bad |= LAYA_STATUS_PAGE;
-              page = p.pages;  // out of bounds: zeros
+          // in the order of use: K 0, K 1, V 0, K 2, V 1, ..., the last V
+          const int ns = r.s1 - r.s0;
+          int page_k = p.prefix_pages[r.s0], page_v[2] = {0, 0};  // of the next K, and of the V that are behind it
+          for (int x = 0, jk = 0, jv = 0; x < 2 * ns && live; x++) {
+            const bool is_k = jk < min(ns, jv + 2);
+            int page;
+            if (is_k) {
+              page = page_k;
+              if (++jk < ns) page_k = p.prefix_pages[r.s0 + jk];
+              if (page < 0 || page >= p.pages) {
+                bad |= LAYA_STATUS_PAGE;
+                page = p.pages;  // out of bounds: zeros
+              }
+              page_v[0] = page_v[1];
+              page_v[1] = page;
+            } else {
+              page = jk - jv == 2 ? page_v[0] : page_v[1];
+              jv++;
             }
+            const int st = g % C::NS;
+            if (!wait(&empty[st], ((g / C::NS) & 1) ^ 1)) break;
+            g++;
+            mbar_expect_tx(&full[st], C::STAGE);
+            const void* map = is_k ? &tk : r.s0 + jv == p.steps ? &tv_last : &tv;
 #pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-              const int st = g % C::NS;
-              if (!wait(&empty[st], ((g / C::NS) & 1) ^ 1)) break;
-              g++;
-              mbar_expect_tx(&full[st], C::STAGE);
-              const void* map = kv == 0 ? &tk : s == p.steps - 1 ? &tv_last : &tv;
-#pragma unroll
-              for (int hb = 0; hb < HD / 64; hb++)
-                tma_load_4d(ring + st * C::STAGE + hb * 8192, map, &full[st], hb * 64, 0, r.kvh, page);
-            }
+            for (int hb = 0; hb < HD / 64; hb++)
+              tma_load_4d(ring + st * C::STAGE + hb * 8192, map, &full[st], hb * 64, 0, r.kvh, page);
           }
         }
         // the last use of every stage is over, or after a timeout its copy has
@@ -714,9 +723,9 @@ __global__ void __maxnreg__(kTcRegs)
           if (!wait(q_full, k & 1)) break;
           k++;
           const int ns = r.s1 - r.s0;
-          // scores of the part's page j (ring stage g + 2 j) for tile t
+          // scores of the part's page j for tile t
           auto scores = [&](int j, int t) {
-            const int x = g + 2 * j, st = x % C::NS, buf = (steps_t[t] + (j > 1 ? 1 : j)) & 1;
+            const int x = g + j + max(0, j - 1), st = x % C::NS, buf = (steps_t[t] + (j > 1 ? 1 : j)) & 1;
             if (!wait(&full[st], (x / C::NS) & 1)) return;
             tc_fence_after();
             // descriptors of the later k-steps: the start address field plus a constant
@@ -735,7 +744,7 @@ __global__ void __maxnreg__(kTcRegs)
           for (int j = 0; j < 2 && j < ns; j++)
             for (int t = 0; t < r.tiles; t++) scores(j, t);
           for (int j = 0; j < ns && live; j++) {
-            const int x = g + 2 * j + 1, st = x % C::NS;
+            const int x = g + j + min(ns, j + 2), st = x % C::NS;
             for (int t = 0; t < r.tiles; t++) {
               const int buf = steps_t[t] & 1;
               if (j == 0) wait(&o_empty[t], (parts_t[t] & 1) ^ 1);
