@@ -104,6 +104,12 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
   return ((x & 0x7fff7fffu) + (__is_same(E, half) ? 0x04000400u : 0x00800080u)) & 0x80008000u;
 }
 
+__device__ __forceinline__ void st_global_8(float* p, const float (&x)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+               "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
+
 // Byte offset of 16-byte piece c of row r in a [HD / 64 blocks][R rows][128 B]
 // tile with 128-byte swizzle.
 template <int R>
@@ -566,8 +572,7 @@ struct Ptc {
   static constexpr int STAGE = 64 * HD * 2;    // K or V of a page: [HD / 64][64 rows][128 B]
   static constexpr int NS = HD == 256 ? 4 : HD == 64 ? 10 : NT == 1 ? 6 : 5;
   static constexpr int OFF_RING = NT * Q_TILE;
-  static constexpr int OFF_OUT = OFF_RING + NS * STAGE;  // 1 KB per softmax warp: 32 rows x 8 F32, coalesced partials
-  static constexpr int OFF_BAR = OFF_OUT + NT * 4 * 1024;
+  static constexpr int OFF_BAR = OFF_RING + NS * STAGE;
   static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 7 * NT) * 8 + 16 + 1024;
   static constexpr int THREADS = 128 + NT * 128;
   static constexpr int COLS = NT * (128 + HD) <= 256 ? 256 : 512;
@@ -878,37 +883,21 @@ __global__ void __maxnreg__(kTcRegs)
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const size_t th = (size_t)tok * p.H + h, rowsH = (size_t)p.rows * p.H;
         if (valid) p.part_l[r.plane * rowsH + th] = log2_sum(mref, l);
-        // A lane holds a row; through shared memory two lanes write 32 bytes of one
-        // (16-byte pieces, piece j of row i at j ^ (i / 4 % 2)).
-        uint4* stage = reinterpret_cast<uint4*>(sm + C::OFF_OUT) + (warp - 4) * 64;
-        const int mine = valid ? (int)th : -1;
-        int rows2[2];  // the rows lane / 2 and lane / 2 + 16, which this lane writes
-#pragma unroll
-        for (int i = 0; i < 2; i++) rows2[i] = __shfl_sync(0xffffffffu, mine, i * 16 + lane / 2);
-        float* dst = p.part_o + r.plane * rowsH * HD + (lane & 1) * 4;
+        // a lane holds a row: 32 bytes, a whole sector, per store
+        float* dst = p.part_o + (r.plane * rowsH + th) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; c++) {
           uint32_t o[32];
           __syncwarp();
           tmem_ld32(tO + c * 32, o);
           tmem_ld_wait();
+          if (valid) {
 #pragma unroll
-          for (int b = 0; b < 4; b++) {
-            __syncwarp();
+            for (int b = 0; b < 32; b += 8) {
+              float x[8];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-              const uint32_t* x = o + 8 * b + 4 * j;
-              stage[lane * 2 + (j ^ (lane >> 2 & 1))] = make_uint4(
-                  __float_as_uint(__uint_as_float(x[0]) * inv), __float_as_uint(__uint_as_float(x[1]) * inv),
-                  __float_as_uint(__uint_as_float(x[2]) * inv), __float_as_uint(__uint_as_float(x[3]) * inv));
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int at_row = i * 16 + lane / 2;
-              const uint4 x = stage[at_row * 2 + ((lane & 1) ^ (at_row >> 2 & 1))];
-              if (rows2[i] >= 0)
-                *reinterpret_cast<uint4*>(dst + (size_t)rows2[i] * HD + c * 32 + b * 8) = x;
+              for (int i = 0; i < 8; i++) x[i] = __uint_as_float(o[b + i]) * inv;
+              st_global_8(dst + c * 32 + b, x);
             }
           }
         }
