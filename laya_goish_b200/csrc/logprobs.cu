@@ -326,7 +326,7 @@ __device__ __forceinline__ float logprob_of(float x, float M, float ln_s) {
 }
 
 struct LpShared {
-  __align__(16) uint32_t seg[kMaxSeg];  // order keys of the segments' maxima (the leader's: all of the row)
+  uint32_t seg[kMaxSeg];  // order keys of the segments' maxima (the leader's: all of the row)
   Stat warp[32];
   Stat cta[8];            // the leader's: one per CTA of the cluster
   int sel[LAYA_MAX_TOP];
@@ -340,10 +340,39 @@ struct LpShared {
 // elements (order keys, then indices).
 extern __shared__ __align__(128) uint4 lp_dyn[];
 
+// The kk best of nseg <= 32 Q segments, by one warp: the best of all, kk times
+// (a rank of each segment among all took six times the instructions, which
+// the rows that are still being read miss: 2048 rows of 152064, 5
+// alternatives, 129 us against 125).  The last one's key.
+template <int Q>
+__device__ __forceinline__ uint32_t best_segments(LpShared& sh, int nseg, int kk) {
+  const int lane = threadIdx.x % 32;
+  uint32_t k[Q], best = 0;
+#pragma unroll
+  for (int q = 0; q < Q; q++) k[q] = q * 32 + lane < nseg ? sh.seg[q * 32 + lane] : 0;
+#pragma unroll 1
+  for (int n = 0; n < kk; n++) {
+    best = 0;
+#pragma unroll
+    for (int q = 0; q < Q; q++) best = max(best, k[q]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    int first = kMaxSeg;
+#pragma unroll
+    for (int q = Q - 1; q >= 0; q--)
+      if (k[q] == best) first = q * 32 + lane;
+    first = __reduce_min_sync(0xffffffffu, first);
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+      if (q * 32 + lane == first) k[q] = 0;  // below every key
+    if (lane == 0) sh.sel[n] = first;
+  }
+  return best;
+}
+
 // The `top` best elements of the row, by the leader CTA, all threads.  Run once
 // per row, so written for few instructions rather than few cycles: unrolled, it
 // cost more in instruction fetches than in work.  2048 rows of 152064 in BF16
-// take 130 us with 5 alternatives and 101 without.
+// take 125 us with 5 alternatives and 101 without.
 template <typename T>
 __device__ void pick_top(const LpArgs& p, const Row<T>& row, int nseg, LpShared& sh, float M, float ln_s,
                          long long r) {
@@ -352,19 +381,10 @@ __device__ void pick_top(const LpArgs& p, const Row<T>& row, int nseg, LpShared&
   uint32_t* ckey = reinterpret_cast<uint32_t*>(lp_dyn);
   int* cidx = reinterpret_cast<int*>(ckey + kCand);
   const int kk = min(p.top, nseg);
-  // the rank of each segment among all
-#pragma unroll 1
-  for (int i = tid; i < nseg; i += nt) {
-    const uint32_t ki = sh.seg[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < nseg; j += 4) {  // padded with zeros, which no key is below
-      const uint4 k4 = *reinterpret_cast<const uint4*>(&sh.seg[j]);
-      rank += (k4.x > ki - (j < i)) + (k4.y > ki - (j + 1 < i)) + (k4.z > ki - (j + 2 < i)) + (k4.w > ki - (j + 3 < i));
-    }
-    if (rank < kk) sh.sel[rank] = i;
+  if (warp == 0) {
+    const uint32_t last = nseg <= 256 ? best_segments<8>(sh, nseg, kk) : best_segments<kMaxSeg / 32>(sh, nseg, kk);
     // the last chosen segment's maximum; fewer segments than `top`: everything counts
-    if (rank == kk - 1) sh.t = nseg < p.top ? kNegInfKey : max(ki, kNegInfKey);
+    if (lane == 0) sh.t = nseg < p.top ? kNegInfKey : max(last, kNegInfKey);
   }
   if (tid == 0) sh.n_cand = 0;
   __syncthreads();
@@ -584,7 +604,7 @@ __global__ void __launch_bounds__(RING ? 32 * (kRingWarps + 1) : 256, 4)
     for (int i = 0, c = rank; i < p.stages && c < chunks; i++, c += C) copy_chunk(c, i);
   }
   if (TOP && rank == 0)
-    for (int i = tid; i < (nseg + 3) / 4 * 4; i += blockDim.x) sh.seg[i] = 0;
+    for (int i = tid; i < nseg; i += blockDim.x) sh.seg[i] = 0;
   // the given tokens' logits, early: their latency hides behind the pass
   float xt = 0.f;
   int tok = -1;
@@ -767,10 +787,10 @@ template <typename T>
 int logprobs_go(LpArgs p, const DeviceInfo& di, cudaStream_t st) {
   const int N = Elem<T>::N;
   // Segments: the more, the less is read again for the `top` (top / segments
-  // of the row), the fewer, the cheaper their choice: about eight per
-  // alternative, 128..512; always more than LAYA_MAX_TOP, or one per vector.
+  // of the row), the fewer, the cheaper their choice: eight per alternative, 256
+  // at least; always more than LAYA_MAX_TOP, or one per vector.
   const long long nvec = ((long long)p.vocab + 2 * N - 2) / N;  // with any misalignment
-  const long long most = std::min(kMaxSeg, std::max(128, p.top * 8));
+  const long long most = std::min(kMaxSeg, std::max(256, p.top * 8));
   p.seg_vec = 1;
   while (nvec > p.seg_vec * most) p.seg_vec *= 2;
   // The ring form keeps one maximum per 128 vectors: rows that still give
