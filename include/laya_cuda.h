@@ -364,7 +364,7 @@ int laya_token_logprobs(uint32_t type, const void* logits, int64_t row_stride, i
                         const int32_t* tokens, int64_t token_stride, int n_tokens, int top, float* logprobs,
                         float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, void* stream);
 
-/* ---- timing of the last laya_decide_batch / laya_decode call ---- */
+/* ---- timing of the last laya_decide_batch / laya_decode / laya_score_tokens call ---- */
 typedef struct laya_timing {
   double device_ms;   /* CUDA-event time on the device stream(s), inputs already in HBM; max over devices */
   int64_t launches;   /* kernels launched by the library during the call (all devices) */

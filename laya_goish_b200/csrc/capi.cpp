@@ -207,6 +207,10 @@ int laya_score_tokens(laya_model* h, const int32_t* ids, const int64_t* offsets,
     for (int64_t t = 0; t < total; t++)
       if (ids[t] < 0 || ids[t] >= m.cfg.V) return fail(LAYA_E_INVALID, "invalid token sequence");
     if (top > m.cfg.V) return fail(LAYA_E_INVALID, "more alternatives than the vocabulary holds");
+    for (auto& r : m.reps) {  // devices without a share report nothing
+      r.call_ms = 0;
+      r.launches = r.h2d = r.d2h = 0;
+    }
     const int nd = std::min((int)m.reps.size(), n_seqs);
     if (nd == 1)
       return score_shard(m, m.reps[0], ids, offsets, 0, n_seqs, top, logprobs, entropy, top_ids, top_logprobs);

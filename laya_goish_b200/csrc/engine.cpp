@@ -2,6 +2,7 @@
 // heads and decision rules.  All device work of one replica runs on that
 // replica's stream; the host plans each wave of requests, uploads the plan
 // and enqueues the layer kernels.
+#include "device_ops.h"
 #include "engine.h"
 
 #include <algorithm>
@@ -1468,6 +1469,15 @@ int score_shard(Model& m, Replica& r, const int32_t* ids, const int64_t* off, in
       LAYA_CK(cudaMemcpy(&err, r.err, 4, cudaMemcpyDeviceToHost));
       if (err)
         return fail(LAYA_E_TIMEOUT, "a device-side wait ran out of its budget (code " + std::to_string(err) + ")");
+      // token_logprobs reports in the device operators' status word
+      DeviceInfo di;
+      if ((rc = device_info(&di))) return rc;
+      LAYA_CK(cudaMemcpy(&err, di.status, 4, cudaMemcpyDeviceToHost));
+      if (err & LAYA_STATUS_TIMEOUT) {
+        err &= ~LAYA_STATUS_TIMEOUT;
+        LAYA_CK(cudaMemcpy(di.status, &err, 4, cudaMemcpyHostToDevice));
+        return fail(LAYA_E_TIMEOUT, "a device-side wait ran out of its budget");
+      }
       if (r.prof) prof_collect(r);
       for (int q = 0; q < R; q++)
         if (!std::isfinite(logprobs[first + q])) return fail(LAYA_E_NONFINITE, "non-finite model output");

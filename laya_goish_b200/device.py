@@ -140,7 +140,8 @@ def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, l
     (its new rows are the last ones).  max_q: the most rows of a sequence.
     scale defaults to head_dim ** -0.5.  Returns out; rows of no sequence are
     left as they were (0 in an out made here), rows that see no key give 0.
-    lse ([rows, heads] F32, optional) receives ln sum exp of the scores."""
+    lse ([rows, heads] F32, optional) receives ln sum exp of the scores.  out
+    and lse share no memory with each other or with what the call reads."""
     if not isinstance(pages, KVPages):
         _refuse("pages must be KVPages")
     return _device.prefix_attention(pages._at, pages._device, q, prefix_pages, prefix_len, tables, lens, offsets,
