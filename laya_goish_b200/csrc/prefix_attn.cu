@@ -147,6 +147,8 @@ __device__ __forceinline__ int prefix_splits(const PfxParams& p, int tok, int kv
   return (int)(((u + 1) * p.steps - 1) / p.chunk - u * p.steps / p.chunk) + 1;
 }
 
+constexpr int kOwnRegs = 144;  // of the unit kernel, head_dim 64 and 128
+
 template <int HD, bool SPLITK>
 struct Unit {
   static constexpr int ROWS = SPLITK ? 16 : 64;
@@ -188,7 +190,7 @@ struct Unit {
 // single rows behind 16384 shared keys 180 / 243, where they also find room
 // beside the prefix kernel).
 template <typename E, int HD, bool SPLITK, bool OWN>
-__global__ void __maxnreg__((HD == 256 ? 255 : 168))
+__global__ void __maxnreg__((HD == 256 ? 255 : kOwnRegs))
     prefix_unit_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const PfxParams p) {
   using C = Unit<HD, SPLITK>;
@@ -570,20 +572,25 @@ struct Ptc {
   static constexpr int NT = NT_;
   static constexpr int Q_TILE = 128 * HD * 2;  // [HD / 64][128 rows][128 B]
   static constexpr int STAGE = 64 * HD * 2;    // K or V of a page: [HD / 64][64 rows][128 B]
-  static constexpr int NS = HD == 256 ? 4 : HD == 64 ? 10 : NT == 1 ? 6 : 5;
+  static constexpr int NS = HD == 256 ? 4 : HD == 64 ? (NT == 1 ? 9 : 10) : NT == 1 ? 3 : 5;
   static constexpr int OFF_RING = NT * Q_TILE;
   static constexpr int OFF_BAR = OFF_RING + NS * STAGE;
   static constexpr int SMEM = OFF_BAR + (2 * NS + 3 + 7 * NT) * 8 + 16 + 1024;
   static constexpr int THREADS = 128 + NT * 128;
   static constexpr int COLS = NT * (128 + HD) <= 256 ? 256 : 512;
   static constexpr int S_COL = 0, O_COL = NT * 128;  // tile t: S at 128 t and 128 t + 64, O at O_COL + HD t
+  // Registers per thread and the ring's depth leave the own-keys kernel's CTAs
+  // (a warp per SM quarter, kOwnRegs) room on the SM: one beside two tiles, two
+  // beside one tile (64 rows, 4001 shared keys x 28/4 heads of 128: 21.4 us a
+  // call, against 25 with six stages and one).  head_dim 256 has none anyway.
+  static constexpr int REGS = 112;
+  static constexpr int BESIDE = HD == 256 ? 0 : NT == 2 ? 1 : 2;
   static_assert(O_COL + NT * HD <= COLS, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory per CTA");
+  static_assert(SMEM + 1024 + BESIDE * (Unit<HD, true>::SMEM + 1024) <= 233472, "shared memory per SM");
+  static_assert((THREADS / 128 * REGS + BESIDE * kOwnRegs) * 32 <= 16384, "registers per SM quarter");
 };
 
-// Per thread: leaves an SM quarter, beside three of these warps, room for one of
-// the own-keys kernel's.
-constexpr int kTcRegs = 112;
 
 struct Run {  // a CTA's part of a unit: pages s0 .. s1 - 1
   int kvh, tok0, s0, s1, plane, tiles;
@@ -605,7 +612,7 @@ __device__ __forceinline__ bool run_part(const PfxParams& p, long long& at, long
 }
 
 template <typename E, int HD, int NT>
-__global__ void __maxnreg__(kTcRegs)
+__global__ void __maxnreg__((Ptc<HD, NT>::REGS))
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tv_last,
                      const PfxParams p) {
@@ -1018,11 +1025,14 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   const int pre_pages = (a.prefix_len + 63) / 64;
   s.pre_tiles = (int)((flat + 15) / 16);
   // 16-row tiles on mma.sync read the prefix once per tile, but start and end
-  // sooner than the tensor-core kernel: it takes over where an SM would get more
-  // than about 25 tile-pages of 64 dimensions (us, mma.sync / tcgen05: 32 rows x
-  // 512 keys x 8 kv heads of 64 8.0 / 10.1, 64 x 4000 13.7 / 17.1, 128 x 4000
-  // 19.8 / 18.6, 64 x 16000 33.9 / 26.2; 56 x 16000 x 4 of 128 31.3 / 27.2).
-  s.tc = flat > 16 && (long long)s.pre_tiles * c.kv_heads * pre_pages * (c.head_dim / 64) > 25ll * sms;
+  // sooner than the tensor-core kernel, which takes over at about ten tile-pages
+  // of head_dim 64 per SM.  The square of head_dim counts: a tile's work per page
+  // and how few CTAs an SM holds (a call's us, mma.sync / tcgen05, tile-pages per
+  // SM: 32 x 1000 keys x 32/8 heads of 64 11.1 / 12.2 at 7, 16 x 4000 14.7 / 13.7
+  // at 14; 4 x 2000 x 28/4 of 128 10.6 / 11.1 at 1.7, 16 x 1000 12.8 / 11.1 at 3;
+  // 16 x 1500 x 8/2 of 256 16.2 / 12.0 at 1.3).
+  const long long wide = c.head_dim / 64;
+  s.tc = flat > 16 && (long long)s.pre_tiles * c.kv_heads * pre_pages * wide * wide > 10ll * sms;
   if (pre_pages && !s.tc) {
     // Key splits until the CTAs fill the GPU once, at least two pages each.
     s.sp = (int)std::max(
@@ -1030,10 +1040,11 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   } else if (pre_pages) {
     s.steps = pre_pages;
     // Two tiles per CTA where a CTA has work for a while; one where it has
-    // twelve pages or fewer (64 rows x 4001 keys x 28/4 heads of 128: 25 us
-    // against 28; at 16 pages level; 512 rows x 16384 keys 212 against 178).
+    // sixteen pages or fewer (us, one / two: 80 rows x 4000 keys x 28/4 heads of
+    // 128 20.2 / 25.4, 160 rows 30.9 / 31.9, 640 rows x 1024 x 32/8 of 64 27.9 /
+    // 25.5, 64 rows x 16000 42 / 36).
     const long long tiles = (a.rows + 128 / G - 1) / (128 / G);
-    s.nt = c.head_dim == 256 || tiles * c.kv_heads * pre_pages <= 12ll * sms ? 1 : 2;
+    s.nt = c.head_dim == 256 || tiles * c.kv_heads * pre_pages <= 16ll * sms ? 1 : 2;
     s.unit_tok = s.nt * (128 / G);
     s.n_units = c.kv_heads * ((a.rows + s.unit_tok - 1) / s.unit_tok);
     const long long work = (long long)s.n_units * s.steps;
