@@ -88,13 +88,16 @@ constexpr uint32_t kNegInfKey = 0x007fffffu;  // order_key(-inf)
 
 // 16-byte pieces of a row.  top: the maximum of several (NaNs left out); it and
 // the bound are taken on packed pairs, before widening.  unpack: the values in
-// F32, no less than low() (a NaN stays), which is finite and far enough down
-// that e^(x - M) is 0 at any ordinary M.
+// F32; BOUND: no less than a finite bound (a NaN stays), at which e^(x - M) is 0
+// for every reference M above kBoundFrom.  F16 has no room below its lowest
+// value, -65504: there the bound is that value, and a row whose reference is
+// near it is taken as it is (-inf must not become a value that is there).
 template <typename T>
 struct Elem;
 template <>
 struct Elem<float> {
   static constexpr int N = 4;
+  static constexpr float kBoundFrom = kDeep;
   static __device__ __forceinline__ float one(float x) { return x; }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -115,6 +118,7 @@ struct Elem<float> {
 template <>
 struct Elem<half> {
   static constexpr int N = 8;
+  static constexpr float kBoundFrom = -65000.f;
   static __device__ __forceinline__ float one(half x) { return __half2float(x); }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -138,6 +142,7 @@ struct Elem<half> {
 template <>
 struct Elem<__nv_bfloat16> {
   static constexpr int N = 8;
+  static constexpr float kBoundFrom = kDeep;
   static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -290,7 +295,7 @@ struct Row {
     constexpr int N = Elem<T>::N;
     const float hi = Elem<T>::top(w);
     if (hi > st.m + kSlack) move_up(st, hi);  // also the first value above -inf
-    if (st.m > kDeep) {
+    if (st.m > Elem<T>::kBoundFrom) {
       const float c = st.m * kLog2e;
       const f32x2 l2 = pack(kLog2e, kLog2e), nc = pack(-c, -c);
 #pragma unroll

@@ -798,3 +798,33 @@ def test_attention_many_partial_results(new, prefix, heads, kv, hd, dtype):
     held = [n + 40 * (i % 3) for i, n in enumerate(new)]
     b = Batch(new, held, prefix, heads, kv, hd, dtype, pad=2, seed=prefix)
     b.check(*b.run())
+
+
+# A logit of -inf is a token that is not there, whatever the others hold: rows
+# of the type's lowest value (a mask) and -inf (padding of the vocabulary) alone,
+# short, long and cut over a cluster, the rows' starts aligned and not.  n equal
+# logits: log probability -ln n, entropy ln n.  The sum is n times one number,
+# which is within 2^-22 of e^(x - M) (ex2.approx), added up within n / 128 + 60
+# roundings in a row; ln and the sums with it round a few times more.
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab,there", [(50, 1), (1000, 999), (3001, 64), (32000, 1000), (152064, 70000)])
+@pytest.mark.parametrize("rows", [1, 40, 700])
+def test_logprobs_lowest_values_beside_minus_infinity(rows, vocab, there, dtype):
+    low = torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    for gap in (0, 3):
+        x = torch.full((rows, vocab + gap), -math.inf, device="cuda", dtype=dtype)[:, gap:]
+        ids = torch.stack([torch.randperm(vocab, device="cuda", generator=g)[:there] for _ in range(min(rows, 4))])
+        ids = ids[torch.arange(rows, device="cuda") % ids.shape[0]].sort(-1).values
+        x.scatter_(1, ids, low)
+        t = torch.stack([ids[:, 0], ids[:, -1]], 1).int()
+        got = device.token_logprobs(x, t, top=5)
+        ln = math.log(there)
+        tol = (there / 128 + 60) * 2.0 ** -24 + 2.0 ** -22 + 8 * 2.0 ** -24 * (1 + ln)
+        assert (got.logprobs.double() + ln).abs().max() <= tol
+        assert (got.entropy.double() - ln).abs().max() <= tol
+        assert (got.lse.double() - (low + ln)).abs().max() <= tol + abs(low) * 2.0 ** -23
+        k = min(5, there)
+        assert torch.equal(got.top_ids[:, :k].long(), ids[:, :k]) and (got.top_ids[:, k:] == -1).all()
+        assert (got.top_logprobs[:, :k].double() + ln).abs().max() <= tol
+        assert (got.top_logprobs[:, k:] == -math.inf).all()
