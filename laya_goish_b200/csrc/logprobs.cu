@@ -175,10 +175,12 @@ __device__ __forceinline__ float y_of(float x, float M) {
   const float y = M > kDeep ? fmaf(x, kLog2e, -(M * kLog2e)) : (x - M) * kLog2e;
   return max_nan(y, -200.f);
 }
-// How far sums move from reference `from` up to reference `to`, in log2 units.
+// How far sums move from reference `from` up to reference `to`, in log2 units:
+// the difference of the rounded c that their y are relative to (a contracted
+// product would leave one of them unrounded: 2e-4 off about 3000).
 __device__ __forceinline__ float shift(float from, float to) {
   if (from <= kDeep && to <= kDeep) return (from - to) * kLog2e;
-  return from * kLog2e - to * kLog2e;
+  return __fsub_rn(__fmul_rn(from, kLog2e), __fmul_rn(to, kLog2e));
 }
 
 // The states of a warp's lanes joined, in every lane.

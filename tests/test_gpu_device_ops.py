@@ -828,3 +828,46 @@ def test_logprobs_lowest_values_beside_minus_infinity(rows, vocab, there, dtype)
         assert torch.equal(got.top_ids[:, :k].long(), ids[:, :k]) and (got.top_ids[:, k:] == -1).all()
         assert (got.top_logprobs[:, :k].double() + ln).abs().max() <= tol
         assert (got.top_logprobs[:, k:] == -math.inf).all()
+
+
+def check_logprob_rows(x, tokens, top=0):
+    """Outputs against 64 bits with tolerances that know no offset of the row.
+    y = (x - M) log2 e has two roundings at most (2^-24 of it each, and log2 e
+    itself is 2^-26 off), so a term is within 2^-22 (ex2.approx) + 3 |y| 2^-24
+    of its size; M is at most 6 below the maximum.  A sum of them adds
+    vocab / 128 roundings in a row and, where M moves and states are joined, at
+    most 60 more (a factor ex2.approx each); ln, products and sums with the
+    results add a few units of theirs.  lse has the offset and one rounding."""
+    u = 2.0 ** -24
+    got = device.token_logprobs(x, tokens, top=top)
+    x = x.double().cpu()
+    d = x - x.amax(-1, keepdim=True)
+    e = torch.exp(d)
+    s = e.sum(-1)
+    p = e / s[:, None]
+    far = (p * torch.where(p > 0, d.abs(), torch.zeros_like(d))).sum(-1) + 6  # mean |y| ln 2, at most
+    rel = (x.shape[1] / 128 + 60) * u + 2.0 ** -22 + 6 * far * u  # of the sum, so absolutely of its ln
+    ln = torch.log(s)
+    y = d - ln[:, None]
+    mean = torch.where(p > 0, p * d, torch.zeros_like(d)).sum(-1)
+    assert ((got.entropy.double().cpu() - (ln - mean)).abs() <= 2 * rel * (1 + far) + 8 * u * (ln + far)).all()
+    want = y.gather(1, tokens.long().cpu())
+    tol = rel[:, None] + 8 * u * (want.abs() + ln[:, None] + 6)
+    assert ((got.logprobs.double().cpu() - want).abs() <= tol).all()
+    lse = x.amax(-1) + ln
+    assert ((got.lse.double().cpu() - lse).abs() <= rel + 8 * u * (ln + 6) + 2 * u * lse.abs()).all()
+    if top:
+        order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(got.top_ids.long().cpu(), order)
+        want = y.gather(1, order)
+        assert ((got.top_logprobs.double().cpu() - want).abs() <= rel[:, None] + 8 * u * (want.abs() + ln[:, None] + 6)).all()
+
+
+# A common offset of a row changes nothing but lse.
+@pytest.mark.parametrize("about", [20, -20, 3000, -3000, 30000, -30000, 64000])
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (3, 32000), (500, 32000)])
+def test_logprobs_with_a_common_offset(rows, vocab, about):
+    g = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    x = about + 2.5 * torch.randn((rows, vocab), device="cuda", generator=g)
+    x[1] = about + torch.linspace(-30, 20, vocab, device="cuda")  # the reference moves again and again
+    check_logprob_rows(x, torch.randint(0, vocab, (rows, 2), device="cuda", generator=g, dtype=torch.int32), top=4)
