@@ -357,8 +357,7 @@ int laya_prefix_attention(const laya_kv_pages* cache, const laya_prefix_args* a,
  *   ascending id: top_ids / top_logprobs [rows][top].
  * A logit of -inf is a token that is not there: it is no alternative (id -1,
  * -inf where fewer than `top` are there), and a row of them alone has lse and
- * logprobs -inf and entropy 0.  A row with NaN or +inf gives NaN, ids -1;
- * so may one with a logit above 2e38. */
+ * logprobs -inf and entropy 0.  A row with NaN or +inf gives NaN, ids -1. */
 #define LAYA_MAX_TOP 64
 int laya_token_logprobs(uint32_t type, const void* logits, int64_t row_stride, int rows, int vocab,
                         const int32_t* tokens, int64_t token_stride, int n_tokens, int top, float* logprobs,

@@ -5,7 +5,8 @@
 //   y = fl(x log2 e - c) (one FMA),  s = sum 2^y,  a = sum 2^y y,
 //   lse = c ln 2 + ln s,  logprob_j = y_j ln 2 - ln s,  entropy = ln s - ln 2 a / s.
 // c's own rounding is the same in every term and cancels; y has one rounding,
-// relative to y itself.  Every thread keeps its own (M, s, a) and moves M only
+// relative to y itself.  (From |M| = 65000 on, y = fl((x - M) log2 e), and M
+// takes the place of c ln 2.)  Every thread keeps its own (M, s, a) and moves M only
 // when a value passes it by more than 6 (terms of up to e^6 cost no precision in
 // F32), so the rescale is rare; the threads' states are merged at the end.
 //
@@ -72,9 +73,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 6.f;
-// Below this, x log2 e may leave F32: a reference there (a row of the type's
-// lowest values) has y = (x - M) log2 e instead.
-constexpr float kDeep = -1e30f;
+// References for which y = fl(x log2 e - c), with c = fl(M log2 e) off by less
+// than 2^-7.  Farther out that error grows past what 2^y can hold (half an ulp
+// of M log2 e is 512 at 1e10), and y = fl((x - M) log2 e) instead: so is a row
+// of masked tokens alone (-1e10, the type's lowest value) or of large logits.
+constexpr float kNear = 65000.f;
+__device__ __forceinline__ bool near(float M) { return fabsf(M) < kNear; }
+// Stands for smaller values of F32 and BF16 at a near reference: e^(x - M) is 0.
+constexpr float kFloor = -1e30f;
 
 // u32 of the same order; -0 counts as +0
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -89,15 +95,12 @@ constexpr uint32_t kNegInfKey = 0x007fffffu;  // order_key(-inf)
 // 16-byte pieces of a row.  top: the maximum of several (NaNs left out); it and
 // the bound are taken on packed pairs, before widening.  unpack: the values in
 // F32; BOUND: no less than a finite bound (a NaN stays), at which e^(x - M) is 0
-// for every reference M above kBoundFrom.  F16 has no room below its lowest
-// value, -65504: there the bound is that value, and a row whose reference is
-// near it is taken as it is (-inf must not become a value that is there).
+// for every near reference M: -65504 for F16, 504 below the lowest of them.
 template <typename T>
 struct Elem;
 template <>
 struct Elem<float> {
   static constexpr int N = 4;
-  static constexpr float kBoundFrom = kDeep;
   static __device__ __forceinline__ float one(float x) { return x; }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -112,13 +115,12 @@ struct Elem<float> {
   static __device__ __forceinline__ void unpack(uint4 v, float (&o)[4]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = BOUND ? max_nan(__uint_as_float(w[i]), kDeep) : __uint_as_float(w[i]);
+    for (int i = 0; i < 4; i++) o[i] = BOUND ? max_nan(__uint_as_float(w[i]), kFloor) : __uint_as_float(w[i]);
   }
 };
 template <>
 struct Elem<half> {
   static constexpr int N = 8;
-  static constexpr float kBoundFrom = -65000.f;
   static __device__ __forceinline__ float one(half x) { return __half2float(x); }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -142,7 +144,6 @@ struct Elem<half> {
 template <>
 struct Elem<__nv_bfloat16> {
   static constexpr int N = 8;
-  static constexpr float kBoundFrom = kDeep;
   static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
   template <int NV>
   static __device__ __forceinline__ float top(const uint4 (&w)[NV]) {
@@ -158,7 +159,7 @@ struct Elem<__nv_bfloat16> {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 x = BOUND ? __hmax2_nan(h[i], __float2bfloat162_rn(kDeep)) : h[i];
+      const __nv_bfloat162 x = BOUND ? __hmax2_nan(h[i], __float2bfloat162_rn(kFloor)) : h[i];
       const uint32_t u = *reinterpret_cast<const uint32_t*>(&x);
       o[2 * i] = __uint_as_float(u << 16);
       o[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
@@ -172,15 +173,16 @@ struct Stat {
 // y of x at reference M; -200 for what is too small to count (2^-200 is 0 in
 // F32), which keeps 0 * inf out of the weighted sum; a NaN stays.
 __device__ __forceinline__ float y_of(float x, float M) {
-  const float y = M > kDeep ? fmaf(x, kLog2e, -(M * kLog2e)) : (x - M) * kLog2e;
+  const float y = near(M) ? fmaf(x, kLog2e, -(M * kLog2e)) : (x - M) * kLog2e;
   return max_nan(y, -200.f);
 }
 // How far sums move from reference `from` up to reference `to`, in log2 units:
-// the difference of the rounded c that their y are relative to (a contracted
-// product would leave one of them unrounded: 2e-4 off about 3000).
+// between near ones the difference of the rounded c that their y are relative to
+// (a contracted product would leave one unrounded: 6e-5 off about 3000).
 __device__ __forceinline__ float shift(float from, float to) {
-  if (from <= kDeep && to <= kDeep) return (from - to) * kLog2e;
-  return __fsub_rn(__fmul_rn(from, kLog2e), __fmul_rn(to, kLog2e));
+  const float c0 = __fmul_rn(from, kLog2e), c1 = __fmul_rn(to, kLog2e);
+  if (near(from)) return near(to) ? __fsub_rn(c0, c1) : -fmaf(to, kLog2e, -c0);
+  return near(to) ? fmaf(from, kLog2e, -c1) : (from - to) * kLog2e;
 }
 
 // The states of a warp's lanes joined, in every lane.
@@ -297,7 +299,7 @@ struct Row {
     constexpr int N = Elem<T>::N;
     const float hi = Elem<T>::top(w);
     if (hi > st.m + kSlack) move_up(st, hi);  // also the first value above -inf
-    if (st.m > Elem<T>::kBoundFrom) {
+    if (near(st.m)) {
       const float c = st.m * kLog2e;
       const f32x2 l2 = pack(kLog2e, kLog2e), nc = pack(-c, -c);
 #pragma unroll
@@ -314,7 +316,7 @@ struct Row {
           st.a = fma2(e, y, st.a);
         }
       }
-    } else {  // nothing seen yet but -inf or the type's lowest values
+    } else {  // nothing seen yet but -inf, or a far reference
 #pragma unroll
       for (int q = 0; q < NV; q++) {
         float x[N];
@@ -328,7 +330,7 @@ struct Row {
 
 __device__ __forceinline__ float logprob_of(float x, float M, float ln_s) {
   // as y_of, but a far smaller logit keeps its distance
-  const float d = M > kDeep && x > kDeep ? fmaf(x, kLog2e, -(M * kLog2e)) * kLn2 : x - M;
+  const float d = near(M) && x > kFloor ? fmaf(x, kLog2e, -(M * kLog2e)) * kLn2 : x - M;
   return d - ln_s;
 }
 
@@ -738,8 +740,8 @@ __global__ void __launch_bounds__(RING ? 32 * (kRingWarps + 1) : 256, 4)
   const float M = bad ? NAN : st.m;
   const float ln_s = none ? 0.f : logf(st.s);
   if (tid == 0) {
-    // the reference is c ln 2: M, and what rounding M log2 e left out
-    const float rest = M > kDeep ? fmaf(-M, kLog2e, M * kLog2e) * kLn2 : 0.f;
+    // a near reference is c ln 2: M, and what rounding M log2 e left out
+    const float rest = near(M) ? fmaf(-M, kLog2e, M * kLog2e) * kLn2 : 0.f;
     if (p.lse) p.lse[r] = none ? -INFINITY : bad ? NAN : M + (ln_s + rest);
     if (p.ent) p.ent[r] = none ? 0.f : bad ? NAN : ln_s - kLn2 * (st.a / st.s);
   }

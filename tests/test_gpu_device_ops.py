@@ -871,3 +871,20 @@ def test_logprobs_with_a_common_offset(rows, vocab, about):
     x = about + 2.5 * torch.randn((rows, vocab), device="cuda", generator=g)
     x[1] = about + torch.linspace(-30, 20, vocab, device="cuda")  # the reference moves again and again
     check_logprob_rows(x, torch.randint(0, vocab, (rows, 2), device="cuda", generator=g, dtype=torch.int32), top=4)
+
+
+# Rows about large values: masked throughout (-1e10), or logits that big; about
+# the values where the arithmetic changes; up to the type's ends.
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("about", [65000, -65000, 1e5, -1e6, 1e9, 1e10, -1e10, -1e20, 9e29, -1e30, 3e38, -3e38])
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (3, 32000), (500, 32000)])
+def test_logprobs_far_from_zero(rows, vocab, about, dtype):
+    g = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    x = about + 2.5 * torch.randn((rows, vocab), device="cuda", generator=g)
+    x[0] = about  # all the same
+    x[1, ::3] = 0.0  # beside ordinary ones
+    x[2, 1::2] = -math.inf
+    x[2, ::5] = torch.finfo(dtype).min
+    t = torch.randint(0, vocab, (rows, 2), device="cuda", generator=g, dtype=torch.int32)
+    t[2] = 2  # one that is there
+    check_logprob_rows(x.to(dtype), t, top=4)
