@@ -20,6 +20,11 @@ struct DeviceInfo {
 int device_info(DeviceInfo* out);
 // Strides, alignment, sizes and type of a cache description; 0 or LAYA_E_INVALID.
 int check_pages(const laya_kv_pages* c);
+// laya_token_logprobs that reports in `status` (null: the device's word, which
+// belongs to the callers of the operators).
+int token_logprobs(uint32_t type, const void* logits, int64_t row_stride, int rows, int vocab, const int32_t* tokens,
+                   int64_t token_stride, int n_tokens, int top, float* logprobs, float* entropy, float* lse,
+                   int32_t* top_ids, float* top_logprobs, unsigned* status, cudaStream_t st);
 
 // Runs an entry point's body; no C++ exception crosses the C boundary.
 template <typename F>

@@ -1450,9 +1450,9 @@ int score_shard(Model& m, Replica& r, const int32_t* ids, const int64_t* off, in
         if ((rc = gemm(r, P_GEMM_HEAD, EPI_F32, r.hid16.as<half>() + (size_t)q0 * c.d, c.d, r.head16, c.d, a)))
           return rc;
         r.launches++;
-        if ((rc = laya_token_logprobs(LAYA_TYPE_F32, r.flog.p, c.V, mr, c.V, dtok.as<int32_t>() + q0, 1, 1, top,
-                                      lp + q0, ent + q0, nullptr, top ? tid + (size_t)q0 * top : nullptr,
-                                      top ? tlp + (size_t)q0 * top : nullptr, r.stream)))
+        if ((rc = token_logprobs(LAYA_TYPE_F32, r.flog.p, c.V, mr, c.V, dtok.as<int32_t>() + q0, 1, 1, top, lp + q0,
+                                 ent + q0, nullptr, top ? tid + (size_t)q0 * top : nullptr,
+                                 top ? tlp + (size_t)q0 * top : nullptr, r.err, r.stream)))
           return rc;
       }
       if ((rc = timing_mark_end(r))) return rc;
@@ -1469,15 +1469,6 @@ int score_shard(Model& m, Replica& r, const int32_t* ids, const int64_t* off, in
       LAYA_CK(cudaMemcpy(&err, r.err, 4, cudaMemcpyDeviceToHost));
       if (err)
         return fail(LAYA_E_TIMEOUT, "a device-side wait ran out of its budget (code " + std::to_string(err) + ")");
-      // token_logprobs reports in the device operators' status word
-      DeviceInfo di;
-      if ((rc = device_info(&di))) return rc;
-      LAYA_CK(cudaMemcpy(&err, di.status, 4, cudaMemcpyDeviceToHost));
-      if (err & LAYA_STATUS_TIMEOUT) {
-        err &= ~LAYA_STATUS_TIMEOUT;
-        LAYA_CK(cudaMemcpy(di.status, &err, 4, cudaMemcpyHostToDevice));
-        return fail(LAYA_E_TIMEOUT, "a device-side wait ran out of its budget");
-      }
       if (r.prof) prof_collect(r);
       for (int q = 0; q < R; q++)
         if (!std::isfinite(logprobs[first + q])) return fail(LAYA_E_NONFINITE, "non-finite model output");

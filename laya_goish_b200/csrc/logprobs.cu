@@ -826,6 +826,29 @@ int logprobs_go(LpArgs p, const DeviceInfo& di, cudaStream_t st) {
 
 }  // namespace
 
+int token_logprobs(uint32_t type, const void* logits, int64_t row_stride, int rows, int vocab, const int32_t* tokens,
+                   int64_t token_stride, int n_tokens, int top, float* logprobs, float* entropy, float* lse,
+                   int32_t* top_ids, float* top_logprobs, unsigned* status, cudaStream_t st) {
+  if (type != LAYA_TYPE_F32 && type != LAYA_TYPE_F16 && type != LAYA_TYPE_BF16)
+    return fail(LAYA_E_INVALID, "logits must be F32, F16 or BF16");
+  if (rows < 0 || vocab < 1 || n_tokens < 0) return fail(LAYA_E_INVALID, "invalid logits size");
+  if (vocab > (1 << 30)) return fail(LAYA_E_INVALID, "vocabulary too large");
+  if (top < 0 || top > LAYA_MAX_TOP) return fail(LAYA_E_INVALID, "top must be 0..64");
+  if (row_stride < 0 || token_stride < 0) return fail(LAYA_E_INVALID, "negative row stride");
+  if (rows == 0) return 0;
+  if (!logits || (n_tokens && (!tokens || !logprobs)) || (top && (!top_ids || !top_logprobs)))
+    return fail(LAYA_E_INVALID, "null argument");
+  if (reinterpret_cast<uintptr_t>(logits) % (type == LAYA_TYPE_F32 ? 4 : 2))
+    return fail(LAYA_E_INVALID, "misaligned logits");
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  LpArgs p{logits,   row_stride, rows, vocab,   tokens,       token_stride, n_tokens,
+           top,      logprobs,   entropy, lse,  top_ids,      top_logprobs, status ? status : di.status, 1, 0};
+  if (type == LAYA_TYPE_F32) return logprobs_go<float>(p, di, st);
+  if (type == LAYA_TYPE_F16) return logprobs_go<half>(p, di, st);
+  return logprobs_go<__nv_bfloat16>(p, di, st);
+}
+
 }  // namespace laya
 
 using namespace laya;
@@ -835,24 +858,7 @@ extern "C" int laya_token_logprobs(uint32_t type, const void* logits, int64_t ro
                                    float* logprobs, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs,
                                    void* stream) {
   return guarded([&]() -> int {
-    if (type != LAYA_TYPE_F32 && type != LAYA_TYPE_F16 && type != LAYA_TYPE_BF16)
-      return fail(LAYA_E_INVALID, "logits must be F32, F16 or BF16");
-    if (rows < 0 || vocab < 1 || n_tokens < 0) return fail(LAYA_E_INVALID, "invalid logits size");
-    if (vocab > (1 << 30)) return fail(LAYA_E_INVALID, "vocabulary too large");
-    if (top < 0 || top > LAYA_MAX_TOP) return fail(LAYA_E_INVALID, "top must be 0..64");
-    if (row_stride < 0 || token_stride < 0) return fail(LAYA_E_INVALID, "negative row stride");
-    if (rows == 0) return 0;
-    if (!logits || (n_tokens && (!tokens || !logprobs)) || (top && (!top_ids || !top_logprobs)))
-      return fail(LAYA_E_INVALID, "null argument");
-    if (reinterpret_cast<uintptr_t>(logits) % (type == LAYA_TYPE_F32 ? 4 : 2))
-      return fail(LAYA_E_INVALID, "misaligned logits");
-    DeviceInfo di;
-    if (int rc = device_info(&di)) return rc;
-    LpArgs p{logits,   row_stride, rows, vocab,   tokens,       token_stride, n_tokens,
-             top,      logprobs,   entropy, lse,  top_ids,      top_logprobs, di.status, 1, 0};
-    auto st = static_cast<cudaStream_t>(stream);
-    if (type == LAYA_TYPE_F32) return logprobs_go<float>(p, di, st);
-    if (type == LAYA_TYPE_F16) return logprobs_go<half>(p, di, st);
-    return logprobs_go<__nv_bfloat16>(p, di, st);
+    return token_logprobs(type, logits, row_stride, rows, vocab, tokens, token_stride, n_tokens, top, logprobs, entropy,
+                          lse, top_ids, top_logprobs, nullptr, static_cast<cudaStream_t>(stream));
   });
 }

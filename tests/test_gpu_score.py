@@ -77,3 +77,30 @@ def test_score_refusals(models):
             e.score_tokens(prompts, top=top)
         assert x.value.code == E_INVALID
     assert e.score_tokens([[3, 4]])[0]["top_ids"].shape == (1, 0)
+
+
+def test_score_leaves_the_operators_status_word_alone(models):
+    """The word in which callers' own operators report (a timeout among them)
+    is neither an error of a scoring call nor cleared by it."""
+    import ctypes
+
+    from laya_goish_b200 import _lib
+
+    e, o = models["tiny-llama-f16"]
+    L = _lib.lib()
+    bits = ctypes.c_uint32()
+    _lib.check(L.laya_device_status(0, ctypes.byref(bits)))
+
+    class Info(ctypes.Structure):  # of the library's own lookup
+        _fields_ = [("device", ctypes.c_int), ("sms", ctypes.c_int), ("status", ctypes.c_uint64)]
+
+    info = Info()
+    assert L._ZN4laya11device_infoEPNS_10DeviceInfoE(ctypes.byref(info)) == 0
+    pending = ctypes.c_uint32(1 | 2)  # a timeout and a page, as kernels of another caller would leave them
+    assert ctypes.CDLL("libcuda.so.1").cuMemcpyHtoD_v2(ctypes.c_uint64(info.status), ctypes.byref(pending),
+                                                       ctypes.c_size_t(4)) == 0
+    try:
+        got = e.score_tokens([[3, 4, 5, 6]], top=2)[0]
+    finally:
+        _lib.check(L.laya_device_status(0, ctypes.byref(bits)))
+    assert np.isfinite(got["logprobs"]).all() and bits.value == 3
