@@ -8,7 +8,11 @@
 
 namespace laya {
 
-__device__ unsigned g_device_status;
+__device__ unsigned g_device_status, g_status_taken;
+
+// Reads and clears the status word in one step: a kernel that sets a bit
+// meanwhile, on any stream, has it in this reading or the next.
+__global__ void take_status_kernel() { g_status_taken = atomicExch(&g_device_status, 0u); }
 
 int device_info(DeviceInfo* out) {
   constexpr int kMax = 64;
@@ -288,15 +292,19 @@ extern "C" int laya_device_status(int device, uint32_t* bits) {
     int before = 0;
     LAYA_CK(cudaGetDevice(&before));
     LAYA_CK(cudaSetDevice(device));
+    static std::mutex mu;  // g_status_taken is one call's at a time
+    std::lock_guard<std::mutex> lk(mu);
     DeviceInfo di;
     int rc = device_info(&di);
     unsigned got = 0;
     cudaError_t e = cudaSuccess;
     if (!rc) {
       e = cudaDeviceSynchronize();
-      if (e == cudaSuccess) e = cudaMemcpy(&got, di.status, 4, cudaMemcpyDeviceToHost);
-      if (e == cudaSuccess && got) e = cudaMemset(di.status, 0, 4);
-      if (e == cudaSuccess && got) e = cudaDeviceSynchronize();
+      if (e == cudaSuccess) {
+        take_status_kernel<<<1, 1>>>();
+        e = cudaGetLastError();
+      }
+      if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&got, g_status_taken, 4);
     }
     cudaSetDevice(before);
     if (rc) return rc;

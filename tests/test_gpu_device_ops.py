@@ -888,3 +888,52 @@ def test_logprobs_far_from_zero(rows, vocab, about, dtype):
     t = torch.randint(0, vocab, (rows, 2), device="cuda", generator=g, dtype=torch.int32)
     t[2] = 2  # one that is there
     check_logprob_rows(x.to(dtype), t, top=4)
+
+
+def test_status_bits_set_while_the_word_is_read_are_not_lost():
+    """One thread reads the status word again and again, with a token bit to
+    clear each time; another sets the page bit 2000 times, at some place of a
+    reading, and waits until a reading has it."""
+    import random
+    import sys
+    import threading
+    import time
+
+    k, v = make_pages(1, 1, 64, F16, False, fill=0.0)
+    pages, row, outside = device.KVPages(k, v), torch.ones((1, 1, 64), device="cuda", dtype=F16), i64([1 << 20])
+    x, bad = torch.zeros((1, 8), device="cuda"), i32([[99]])
+    side = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    seen, stop = [0], threading.Event()
+
+    def reader():
+        while not stop.is_set():
+            with torch.cuda.stream(side[1]):
+                device.token_logprobs(x, bad)
+            seen[0] |= status_bits() & 2
+
+    t = threading.Thread(target=reader)
+    t.start()
+    lost, r, interval = 0, random.Random(1), sys.getswitchinterval()
+    try:
+        sys.setswitchinterval(1e-6)  # both threads run all the while
+        for _ in range(2000):
+            until = time.perf_counter() + 3e-4 * r.random()
+            while time.perf_counter() < until:
+                pass
+            seen[0] = 0
+            with torch.cuda.stream(side[0]):
+                device.kv_append(pages, row, row, outside)
+            side[0].synchronize()
+            until = time.monotonic() + 2
+            while not seen[0] and time.monotonic() < until:
+                pass
+            if not seen[0]:
+                lost += 1
+                break
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        t.join()
+        status_bits()
+    assert not lost
