@@ -332,7 +332,7 @@ typedef struct laya_prefix_args {
   const int32_t* offsets;       /* n_seqs + 1, ascending */
   int32_t n_seqs, max_q;        /* max_q: the most query rows of a sequence (rows past it are not computed) */
   const int32_t* prefix_pages;  /* ceil(prefix_len / 64) pages */
-  int32_t prefix_len;
+  int32_t prefix_len;           /* prefix_len and width * 64 at most 2^31 - 64 */
   int32_t width;
   const int32_t* tables;
   int64_t table_stride;

@@ -34,6 +34,7 @@ namespace {
 
 constexpr long long kBudget = 400000000ll;  // SM cycles per bounded wait (~0.2 s)
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxKeys = 0x7fffffff - 63;
 
 struct PfxParams {
   const void* q;
@@ -1019,7 +1020,8 @@ struct Shape {
 Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   Shape s{};
   const int G = a.heads / c.kv_heads;
-  const long long flat = (long long)a.rows * G, own_flat = (long long)a.max_q * G;
+  // no sequence has more rows than there are, however loose the caller's bound
+  const long long flat = (long long)a.rows * G, own_flat = (long long)std::min(a.max_q, a.rows) * G;
   s.own_split = own_flat <= 16;
   s.own_tiles = (int)((own_flat + (s.own_split ? 16 : 64) - 1) / (s.own_split ? 16 : 64));
   const int pre_pages = (a.prefix_len + 63) / 64;
@@ -1073,6 +1075,9 @@ int check_sizes(const laya_kv_pages* c, const laya_prefix_args* a) {
   if (a->heads < 1 || a->heads % c->kv_heads) return fail(LAYA_E_INVALID, "heads must be a multiple of kv_heads");
   if (a->heads / c->kv_heads > 128) return fail(LAYA_E_INVALID, "more than 128 query heads per kv head");
   if ((long long)a->rows * a->heads > 0x7fffffffll) return fail(LAYA_E_INVALID, "too many query rows");
+  // positions up to the end of the last page are 32-bit
+  if (a->prefix_len > kMaxKeys || a->width > kMaxKeys / 64)
+    return fail(LAYA_E_INVALID, "prefix_len or width beyond 2^31 - 64 keys");
   return 0;
 }
 

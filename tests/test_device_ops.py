@@ -152,3 +152,16 @@ def test_host_tensors_are_refused():
             call()
     with pytest.raises(_lib.LayaError, match="KVPages"):
         device.kv_append(None, x, x, t)
+
+
+def test_prefix_attention_refuses_keys_beyond_32_bit_positions():
+    L = _lib.lib()
+    good = dict(q=A, q_stride=2048, rows=3, heads=32, offsets=A, n_seqs=2, max_q=2, prefix_pages=A, prefix_len=100,
+                width=2, tables=A, table_stride=1 << 30, lens=A, scale=0.125, out=A, out_stride=2048)
+    most = (1 << 31) - 64
+    for change in (dict(prefix_len=most + 1), dict(prefix_len=(1 << 31) - 1), dict(width=most // 64 + 1)):
+        a = _lib.PrefixArgs(**dict(good, **change))
+        invalid(L.laya_prefix_attention(ctypes.byref(cache()), ctypes.byref(a), None), "2^31 - 64 keys")
+        assert L.laya_prefix_attention_workspace(ctypes.byref(cache()), ctypes.byref(a)) == 0
+    a = _lib.PrefixArgs(**dict(good, prefix_len=most, width=most // 64, rows=0))
+    assert L.laya_prefix_attention(ctypes.byref(cache()), ctypes.byref(a), None) == 0

@@ -937,3 +937,18 @@ def test_status_bits_set_while_the_word_is_read_are_not_lost():
         t.join()
         status_bits()
     assert not lost
+
+
+# max_q is a bound: one as loose as a context length, or the largest there is,
+# changes neither results nor what is accepted.
+@pytest.mark.parametrize("bound", [7, 70, 100000, 2 ** 31 - 1])
+@pytest.mark.parametrize("new,prefix", [([1, 1, 1], 0), ([1, 1, 1], 130), ([3, 0, 1], 700), ([70, 2], 100)])
+def test_attention_with_a_loose_bound_of_rows(new, prefix, bound):
+    b = Batch(new, [n + 50 for n in new], prefix, 8, 2, 64, F16, pad=3, seed=prefix + len(new))
+    b.check(*b.run(max_q=max(bound, max(new))))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_attention_of_the_widest_groups_with_the_largest_bound(rows):
+    b = Batch([1] * rows, [9] * rows, 70, 128, 1, 64, F16, seed=rows)
+    b.check(*b.run(max_q=2 ** 31 - 1))
