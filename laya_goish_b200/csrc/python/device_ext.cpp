@@ -81,6 +81,7 @@ const at::Tensor& tensor(PyObject* o, const char* name, int64_t dim, int type, i
   if (device != kAny && t.get_device() != device) refuse(std::string(name) + " is on another device");
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse(std::string(name) + " requires a gradient; the operators are forward only");
+  if (t._fw_grad(0).defined()) refuse(std::string(name) + " has a tangent; the operators are forward only");
   if (t.is_conj() || t.is_neg()) refuse(std::string(name) + " must not be a lazily negated view");
   return t;
 }
@@ -183,15 +184,23 @@ const laya_kv_pages* pages_at(PyObject* o) {
   return static_cast<const laya_kv_pages*>(p);
 }
 
-// (pages address, device, k, v, slots)
+// The tensors behind the pages, which may have come to require a gradient
+// since the pages were described.
+void page_tensors(const laya_kv_pages* c, PyObject* k, PyObject* v, int device) {
+  tensor(k, "k pages", 4, (int)scalar_type(c->type), device);
+  tensor(v, "v pages", 4, (int)scalar_type(c->type), device);
+}
+
+// (pages address, device, pages' k, pages' v, k, v, slots)
 PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
-    arguments(na, 5);
+    arguments(na, 7);
     const laya_kv_pages* c = pages_at(a[0]);
     const int dev = (int)integer(a[1], "device", 0, INT32_MAX);
-    const at::Tensor& k = tensor(a[2], "k", 3, kAny, dev);
-    const at::Tensor& v = tensor(a[3], "v", 3, (int)k.scalar_type(), dev);
-    const at::Tensor& slots = flat(a[4], "slots", (int)at::kLong, dev);
+    page_tensors(c, a[2], a[3], dev);
+    const at::Tensor& k = tensor(a[4], "k", 3, kAny, dev);
+    const at::Tensor& v = tensor(a[5], "v", 3, (int)k.scalar_type(), dev);
+    const at::Tensor& slots = flat(a[6], "slots", (int)at::kLong, dev);
     if (k.scalar_type() != scalar_type(c->type) && k.scalar_type() != at::kFloat)
       refuse("k and v must be of the pages' type or F32");
     if (k.sizes() != v.sizes() || k.size(0) != slots.size(0) || k.size(1) != c->kv_heads || k.size(2) != c->head_dim)
@@ -203,43 +212,44 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
-// (pages address, device, q, prefix_pages, prefix_len, tables, lens, offsets, max_q, scale or None, out or None, lse or None)
+// (pages address, device, pages' k, pages' v, q, prefix_pages, prefix_len, tables, lens, offsets, max_q, scale or None, out or None, lse or None)
 PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
-    arguments(na, 12);
+    arguments(na, 14);
     const laya_kv_pages* c = pages_at(a[0]);
     const int dev = (int)integer(a[1], "device", 0, INT32_MAX);
+    page_tensors(c, a[2], a[3], dev);
     const at::ScalarType type = scalar_type(c->type);
-    const at::Tensor& q = tensor(a[2], "q", 3, (int)type, dev);
-    const at::Tensor& prefix_pages = flat(a[3], "prefix_pages", (int)at::kInt, dev);
-    const at::Tensor& tables = tensor(a[5], "tables", 2, (int)at::kInt, dev);
-    const at::Tensor& lens = flat(a[6], "lens", (int)at::kInt, dev);
-    const at::Tensor& offsets = flat(a[7], "offsets", (int)at::kInt, dev);
+    const at::Tensor& q = tensor(a[4], "q", 3, (int)type, dev);
+    const at::Tensor& prefix_pages = flat(a[5], "prefix_pages", (int)at::kInt, dev);
+    const at::Tensor& tables = tensor(a[7], "tables", 2, (int)at::kInt, dev);
+    const at::Tensor& lens = flat(a[8], "lens", (int)at::kInt, dev);
+    const at::Tensor& offsets = flat(a[9], "offsets", (int)at::kInt, dev);
     const int64_t n = tables.size(0), width = tables.size(1), rows = q.size(0), heads = q.size(1), hd = q.size(2);
     if (hd != c->head_dim) refuse("q and the pages have different head_dim");
     if (!heads || heads % c->kv_heads) refuse("heads must be a multiple of kv_heads");
     if (lens.size(0) != n || offsets.size(0) != n + 1) refuse("lens, offsets and tables must fit the sequences");
     if (n && width > 1 && tables.stride(1) != 1) refuse("the rows of tables must be contiguous");
     laya_prefix_args p{};
-    p.prefix_len = (int32_t)integer(a[4], "prefix_pages must hold prefix_len tokens: prefix_len", 0, INT32_MAX);
+    p.prefix_len = (int32_t)integer(a[6], "prefix_pages must hold prefix_len tokens: prefix_len", 0, INT32_MAX);
     if (p.prefix_len > prefix_pages.size(0) * LAYA_PAGE_TOKENS) refuse("prefix_pages must hold prefix_len tokens");
-    p.max_q = (int32_t)integer(a[8], "max_q", 0, INT32_MAX);
-    if (a[9] == Py_None) {
+    p.max_q = (int32_t)integer(a[10], "max_q", 0, INT32_MAX);
+    if (a[11] == Py_None) {
       p.scale = (float)(1.0 / std::sqrt((double)hd));
     } else {
-      const double s = PyFloat_AsDouble(a[9]);
+      const double s = PyFloat_AsDouble(a[11]);
       if (s == -1.0 && PyErr_Occurred()) throw Refused{};
       p.scale = (float)s;
     }
     c10::cuda::CUDAGuard guard(dev);
     at::AutoDispatchBelowADInplaceOrView below;
-    const bool given = a[10] != Py_None;
+    const bool given = a[12] != Py_None;
     at::Tensor made;
     if (!given) made = at::zeros(q.sizes(), q.options());
-    const at::Tensor& out = given ? tensor(a[10], "out", 3, (int)type, dev) : made;
+    const at::Tensor& out = given ? tensor(a[12], "out", 3, (int)type, dev) : made;
     if (out.sizes() != q.sizes()) refuse("out must have q's shape");
-    if (a[11] != Py_None) {
-      const at::Tensor& lse = tensor(a[11], "lse", 2, (int)at::kFloat, dev);
+    if (a[13] != Py_None) {
+      const at::Tensor& lse = tensor(a[13], "lse", 2, (int)at::kFloat, dev);
       if (lse.size(0) != rows || lse.size(1) != heads || !lse.is_contiguous())
         refuse("lse must be contiguous [rows, heads]");
       p.lse = ptr<float>(lse);
@@ -265,8 +275,8 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     }
     check(laya_prefix_attention(c, &p, stream_of(dev)));
     if (!given) return THPVariable_Wrap(made);
-    Py_INCREF(a[10]);
-    return a[10];
+    Py_INCREF(a[12]);
+    return a[12];
   });
 }
 

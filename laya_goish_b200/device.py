@@ -11,8 +11,9 @@ captured into a CUDA graph (after a first call on the device).  Nothing is
 kept between calls: outputs and workspaces come from torch's allocator.  What
 is wrong with the arguments raises LayaError ("invalid"); what only the GPU
 sees (page numbers, slots, lengths, token ids out of range) is skipped by the
-kernels and reported by ``check_status``.  Forward only.  There is no
-counterpart in the reference, which has no K/V cache.
+kernels and reported by ``check_status``.  Forward only: tensors that require a
+gradient (while gradients are recorded) or have a tangent are refused.  There
+is no counterpart in the reference, which has no K/V cache.
 """
 from __future__ import annotations
 
@@ -129,7 +130,7 @@ def kv_append(pages: KVPages, k, v, slots) -> None:
     distinct)."""
     if not isinstance(pages, KVPages):
         _refuse("pages must be KVPages")
-    _device.kv_append(pages._at, pages._device, k, v, slots)
+    _device.kv_append(pages._at, pages._device, pages.k, pages.v, k, v, slots)
 
 
 def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, lens, offsets, max_q: int,
@@ -144,8 +145,8 @@ def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, l
     and lse share no memory with each other or with what the call reads."""
     if not isinstance(pages, KVPages):
         _refuse("pages must be KVPages")
-    return _device.prefix_attention(pages._at, pages._device, q, prefix_pages, prefix_len, tables, lens, offsets,
-                                    max_q, scale, out, lse)
+    return _device.prefix_attention(pages._at, pages._device, pages.k, pages.v, q, prefix_pages, prefix_len, tables,
+                                    lens, offsets, max_q, scale, out, lse)
 
 
 class TokenLogprobs(NamedTuple):

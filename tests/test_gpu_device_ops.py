@@ -952,3 +952,38 @@ def test_attention_with_a_loose_bound_of_rows(new, prefix, bound):
 def test_attention_of_the_widest_groups_with_the_largest_bound(rows):
     b = Batch([1] * rows, [9] * rows, 70, 128, 1, 64, F16, seed=rows)
     b.check(*b.run(max_q=2 ** 31 - 1))
+
+
+def test_no_gradient_is_dropped_without_a_word():
+    """Pages that require a gradient, and forward-mode tangents anywhere, are refused like other inputs with gradients."""
+    from torch.autograd import forward_ad
+
+    b = Batch([1, 2], [64, 64], 100, 8, 2, 64, F16, seed=13)
+    new, slots = torch.zeros((2, 2, 64), device="cuda", dtype=F16), i64([0, 1])
+    x, t = torch.zeros((2, 50), device="cuda"), i32([[0], [0]])
+    for name in ("k", "v"):
+        kv = dict(k=b.k.clone(), v=b.v.clone())
+        kv[name].requires_grad_()
+        pages = device.KVPages(kv["k"], kv["v"])
+        b.pages = pages
+        with pytest.raises(LayaError, match="forward only"):
+            b.run()
+        with pytest.raises(LayaError, match="forward only"):
+            device.kv_append(pages, new, new, slots)
+        with torch.no_grad():
+            b.run()
+            device.kv_append(pages, new, new, slots)
+    pages = b.pages = device.KVPages(b.k, b.v)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(y, torch.ones_like(y)) for y in (b.q, new, x)]
+        with pytest.raises(LayaError, match="tangent"):
+            b.run(q=dual[0])
+        for k, v in ((dual[1], new), (new, dual[1])):
+            with pytest.raises(LayaError, match="tangent"):
+                device.kv_append(pages, k, v, slots)
+        with pytest.raises(LayaError, match="tangent"):
+            device.token_logprobs(dual[2], t)
+        b.pages = device.KVPages(forward_ad.make_dual(b.k, torch.ones_like(b.k)), b.v)
+        with pytest.raises(LayaError, match="tangent"):
+            b.run()
+    device.check_status()
