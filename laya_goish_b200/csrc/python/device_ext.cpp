@@ -123,6 +123,11 @@ template <typename T = void>
 T* ptr(const at::Tensor& t) {
   return static_cast<T*>(t.data_ptr());
 }
+// An in-place write, for autograd: a tensor saved for a backward pass and
+// written since is an error there.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, int device) {
   return at::empty(size, at::TensorOptions().dtype(type).device(at::kCUDA, device));
 }
@@ -174,6 +179,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t na) {
                          size32(free_pages.size(0), "free_pages"), base, ptr<int32_t>(tables), stride,
                          size32(width, "tables"), ptr<int64_t>(slots), ptr<int32_t>(positions), ptr<int32_t>(seqs),
                          capacity, ptr<int32_t>(offsets), ptr<int32_t>(lens), ptr<int64_t>(totals), stream_of(dev)));
+    written(tables);
     return tuple_of({slots, positions, seqs, offsets, lens, totals});
   });
 }
@@ -208,6 +214,8 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     c10::cuda::CUDAGuard guard(dev);
     check(laya_kv_append(c, type_code(k.scalar_type()), ptr(k), ptr(v), rows_of(k, "k"), rows_of(v, "v"),
                          ptr<int64_t>(slots), size32(k.size(0), "rows"), stream_of(dev)));
+    written(THPVariable_Unpack(a[2]));
+    written(THPVariable_Unpack(a[3]));
     Py_RETURN_NONE;
   });
 }
@@ -274,7 +282,9 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
       p.workspace = ptr(work);
     }
     check(laya_prefix_attention(c, &p, stream_of(dev)));
+    if (p.lse) written(THPVariable_Unpack(a[13]));
     if (!given) return THPVariable_Wrap(made);
+    written(out);
     Py_INCREF(a[12]);
     return a[12];
   });

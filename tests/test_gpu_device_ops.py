@@ -987,3 +987,30 @@ def test_no_gradient_is_dropped_without_a_word():
         with pytest.raises(LayaError, match="tangent"):
             b.run()
     device.check_status()
+
+
+def test_writes_are_seen_by_autograd():
+    """What a call writes in place cannot go unnoticed into a backward pass that saved it before."""
+    b = Batch([1, 2], [64, 64], 100, 8, 2, 64, F16, seed=14)
+    new, slots = torch.ones((2, 2, 64), device="cuda", dtype=F16), i64([0, 1])
+    out, lse = torch.zeros_like(b.q), torch.zeros((b.rows, 8), device="cuda")
+
+    def plan():
+        device.page_plan(i32([64, 64]), i32([1, 2]), i32([0, 1]), b.tables, 3)
+
+    for call, tensors in ((lambda: b.run(out=out, lse=lse), (out, lse)),
+                          (lambda: device.kv_append(b.pages, new, new, slots), (b.k, b.v)), (plan, (b.tables,))):
+        for t in tensors:
+            before = t._version
+            call()
+            assert t._version == before + 1
+            if t.is_floating_point():
+                w = torch.ones((), device="cuda", requires_grad=True)
+                loss = (w * t).float().sum()
+                call()
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    loss.backward()
+    with torch.inference_mode():  # inference tensors have no version
+        q = b.q.clone()
+        b.run(q=q, out=torch.zeros_like(q))
+    device.check_status()
