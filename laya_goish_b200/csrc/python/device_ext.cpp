@@ -190,11 +190,12 @@ const laya_kv_pages* pages_at(PyObject* o) {
   return static_cast<const laya_kv_pages*>(p);
 }
 
-// The tensors behind the pages, which may have come to require a gradient
-// since the pages were described.
+// The tensors behind the pages, which may have come to require a gradient, or
+// been given other memory, since the pages were described.
 void page_tensors(const laya_kv_pages* c, PyObject* k, PyObject* v, int device) {
-  tensor(k, "k pages", 4, (int)scalar_type(c->type), device);
-  tensor(v, "v pages", 4, (int)scalar_type(c->type), device);
+  const at::Tensor& tk = tensor(k, "k pages", 4, (int)scalar_type(c->type), device);
+  const at::Tensor& tv = tensor(v, "v pages", 4, (int)scalar_type(c->type), device);
+  if (tk.data_ptr() != c->k || tv.data_ptr() != c->v) refuse("the pages' tensors have moved since KVPages was made");
 }
 
 // (pages address, device, pages' k, pages' v, k, v, slots)

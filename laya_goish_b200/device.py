@@ -85,7 +85,8 @@ def page_plan(past, count, free_pages, tables, capacity: int, base: int = 0) -> 
 class KVPages:
     """One layer's K and V pages, k and v [pages, kv_heads, 64, head_dim] F16 or
     BF16 with equal strides: the engine's layout, or a permuted view of pages
-    held token by token ([pages, 64, kv_heads, head_dim].permute(0, 2, 1, 3))."""
+    held token by token ([pages, 64, kv_heads, head_dim].permute(0, 2, 1, 3)).
+    Tensors that are given other memory afterwards need a new one."""
 
     def __init__(self, k, v):
         _pages(k, "k pages")

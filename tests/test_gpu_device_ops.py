@@ -1014,3 +1014,18 @@ def test_writes_are_seen_by_autograd():
         q = b.q.clone()
         b.run(q=q, out=torch.zeros_like(q))
     device.check_status()
+
+
+def test_pages_whose_tensors_moved_are_refused():
+    for name in ("k", "v"):
+        b = Batch([1, 2], [64, 64], 100, 8, 2, 64, F16, seed=15)
+        t = getattr(b, name)
+        old = t.data  # keeps the old memory alive
+        new, slots = torch.ones((2, 2, 64), device="cuda", dtype=F16), i64([0, 1])
+        t.data = old.clone()
+        with pytest.raises(LayaError, match="moved"):
+            b.run()
+        with pytest.raises(LayaError, match="moved"):
+            device.kv_append(b.pages, new, new, slots)
+        b.pages = device.KVPages(b.k, b.v)
+        b.check(*b.run())
