@@ -1,5 +1,6 @@
 """Builds liblaya_cuda.so in-tree for sm_100a (nvcc cross-compiles without a GPU),
-and _device.so, the Python binding of the operators on torch tensors.
+and, where torch is installed, _device.so, the Python binding of the operators
+on torch tensors.
 
     python -m laya_goish_b200.build          # incremental
     python -m laya_goish_b200.build --clean  # full rebuild
@@ -8,6 +9,8 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -47,12 +50,24 @@ def _compile(src: str) -> str:
     return obj
 
 
-def _compile_ext() -> str:
-    """The binding's object file (torch's headers, the host compiler)."""
-    obj = os.path.join(BUILD, "device_ext.o")
+def _compile_ext() -> str | None:
+    """The binding's object file (torch's headers, the host compiler); None
+    without torch, for which there is nothing to bind.  Built again for another
+    torch or Python, whose ABI may differ."""
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: _device.so is not built", file=sys.stderr)
+        return None
+    obj, stamp = os.path.join(BUILD, "device_ext.o"), os.path.join(BUILD, "device_ext.for")
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a source tree on the path
+        version = "of unknown version"
+    built_for = f"torch {version} {importlib.util.find_spec('torch').origin}\n{sys.version}\n"
     newest = max(os.path.getmtime(f) for f in [EXT_SRC] + glob.glob(os.path.join(INCLUDE, "*.h")))
-    if os.path.exists(obj) and os.path.getmtime(obj) >= newest:
-        return obj
+    if os.path.exists(obj) and os.path.getmtime(obj) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == built_for:
+                return obj
     import torch
     from torch.utils import cpp_extension
 
@@ -64,6 +79,8 @@ def _compile_ext() -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {EXT_SRC}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return obj
 
 
@@ -88,14 +105,15 @@ def build(clean: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         ext = ex.submit(_compile_ext)
         objs = list(ex.map(_compile, _sources()))
-        ext_obj = ext.result()
-    if not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
-        cmd = [NVCC, *ARCH, "-shared", "-o", OUT + ".tmp", *objs, "-lpthread"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-        os.replace(OUT + ".tmp", OUT)
-    _link_ext(ext_obj)
+        if not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
+            cmd = [NVCC, *ARCH, "-shared", "-o", OUT + ".tmp", *objs, "-lpthread"]
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+            os.replace(OUT + ".tmp", OUT)
+    # the library is there whether or not the binding can be
+    if ext_obj := ext.result():
+        _link_ext(ext_obj)
     return OUT
 
 
