@@ -1029,3 +1029,61 @@ def test_pages_whose_tensors_moved_are_refused():
             device.kv_append(b.pages, new, new, slots)
         b.pages = device.KVPages(b.k, b.v)
         b.check(*b.run())
+
+
+def prefix_kernel(rows, heads, kv, hd, prefix):
+    """(row tiles per CTA of the tensor-core kernel or 0 for the other one, row
+    tiles), by the rules that the launch code states."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    group, pages = heads // kv, pages_of(prefix)
+    small = -(-rows * group // 16)
+    if rows * group <= 16 or small * kv * pages * (hd // 64) ** 2 <= 10 * sms:
+        return 0, small
+    tiles = -(-rows // (128 // group))
+    return (1 if hd == 256 or tiles * kv * pages <= 16 * sms else 2), tiles
+
+
+# Two row tiles per CTA and an odd number of them, so that the last CTAs have
+# one; the widest groups (a tile of one token, rows of a tile unused).
+ODD_TILES = [
+    ([1] * 330, 2048, 32, 8, 64),
+    ([11] * 31, 4300, 12, 4, 64),
+    ([1] * 230, 2900, 28, 4, 128),
+    ([3, 5, 200, 0, 110], 3001, 20, 4, 128),
+    ([1] * 21, 8000, 128, 1, 64),
+    ([1] * 24, 6400, 100, 1, 128),
+    ([2, 3], 4000, 65, 1, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(ODD_TILES)))
+def test_attention_tensor_core_odd_tiles_and_wide_groups(case, dtype):
+    new, prefix, heads, kv, hd = ODD_TILES[case]
+    pad = case % 2
+    nt, tiles = prefix_kernel(sum(new) + pad, heads, kv, hd, prefix)
+    assert nt == (1 if hd == 256 else 2) and tiles % 2 == 1
+    b = Batch(new, [n + i % 5 for i, n in enumerate(new)], prefix, heads, kv, hd, dtype, token_major=case % 2 == 0,
+              pad=pad, seed=90 + case)
+    out, lse = b.run()
+    b.check(out, lse)
+    again = b.run()
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+def test_the_tensor_core_cases_reach_both_forms():
+    forms = {hd: set() for hd in (64, 128, 256)}
+    for new, _, prefix, heads, kv, hd in TENSOR_CORE:
+        nt, _ = prefix_kernel(sum(new), heads, kv, hd, prefix)
+        assert nt
+        forms[hd].add(nt)
+    assert forms == {64: {1, 2}, 128: {1, 2}, 256: {1}}
+
+
+@pytest.mark.parametrize("new,held,prefix,heads,kv,hd", [([700], [700], 0, 8, 2, 64), ([513, 1, 1], [600, 90, 1], 70, 4, 2, 128),
+                                                         ([257, 0, 300], [257, 5, 1000], 300, 2, 2, 256),
+                                                         ([40, 2], [50, 2], 0, 128, 1, 64)])
+def test_attention_of_prompts(new, held, prefix, heads, kv, hd):
+    """Many new rows, alone and beside single ones."""
+    b = Batch(new, held, prefix, heads, kv, hd, BF16, pad=1, seed=len(new) + hd)
+    b.check(*b.run())
