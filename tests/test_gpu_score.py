@@ -104,3 +104,22 @@ def test_score_leaves_the_operators_status_word_alone(models):
     finally:
         _lib.check(L.laya_device_status(0, ctypes.byref(bits)))
     assert np.isfinite(got["logprobs"]).all() and bits.value == 3
+
+
+def test_score_in_chunks_of_logits():
+    """More rows than one chunk of logits holds (256 MB), over an odd vocabulary."""
+    path = synth.model_path(synth.Decoder("wide-head-llama-f16", "llama", 1, 256, 4, 2, 512, 40001, 1e4, quant="f16",
+                                          seed=18))
+    e, o = engine.Engine(path), oracle.Model(open(path, "rb").read(), threads=8)
+    rng = np.random.default_rng(8)
+    prompts = [synth.token_ids(rng, o.vocab, n) for n in (900, 1, 700, 333)]  # 1930 rows, 1664 to a chunk
+    for ids, g in zip(prompts, e.score_tokens(prompts, top=3)):
+        if len(ids) < 2:
+            continue
+        lp = log_softmax(np.asarray(o.head(o.forward(ids, list(range(len(ids) - 1)))), np.float64))
+        err = np.abs(g["logprobs"] - lp[np.arange(len(ids) - 1), ids[1:]])
+        assert err.max() < 3e-2 and err.mean() < 3e-3, (err.max(), err.mean())
+        assert np.abs(g["entropy"] + (np.exp(lp) * lp).sum(-1)).max() < 3e-2
+        assert np.abs(np.take_along_axis(lp, g["top_ids"].astype(np.int64), 1) - g["top_logprobs"]).max() < 3e-2
+    e.close()
+    o.close()
