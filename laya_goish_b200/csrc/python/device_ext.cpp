@@ -24,6 +24,7 @@
 namespace {
 
 PyObject* g_error;  // laya_goish_b200._lib.LayaError
+PyObject* g_oom;    // torch.OutOfMemoryError
 
 struct Refused {};  // a Python error is set
 
@@ -46,6 +47,8 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const Refused&) {
+  } catch (const c10::OutOfMemoryError& e) {  // what callers of torch catch
+    PyErr_SetString(g_oom, e.what_without_backtrace());
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
@@ -333,6 +336,10 @@ PyMODINIT_FUNC PyInit__device(void) {
   if (!lib) return nullptr;
   g_error = PyObject_GetAttrString(lib, "LayaError");
   Py_DECREF(lib);
-  if (!g_error) return nullptr;
+  PyObject* torch = g_error ? PyImport_ImportModule("torch") : nullptr;
+  if (!torch) return nullptr;
+  g_oom = PyObject_GetAttrString(torch, "OutOfMemoryError");
+  Py_DECREF(torch);
+  if (!g_oom) return nullptr;
   return PyModule_Create(&g_module);
 }

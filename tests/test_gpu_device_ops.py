@@ -1087,3 +1087,10 @@ def test_attention_of_prompts(new, held, prefix, heads, kv, hd):
     """Many new rows, alone and beside single ones."""
     b = Batch(new, held, prefix, heads, kv, hd, BF16, pad=1, seed=len(new) + hd)
     b.check(*b.run())
+
+
+def test_no_memory_for_the_outputs_is_torch_s_own_error():
+    n = 1 << 30  # rows that share their memory; 64 alternatives of each would take 0.5 TB
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        device.token_logprobs(torch.zeros((1, 8), device="cuda").expand(n, 8), i32([[0]]).expand(n, 1), top=64)
+    device.check_status()
