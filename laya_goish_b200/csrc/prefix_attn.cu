@@ -15,7 +15,13 @@
 // are not split, the own-keys kernel writes the output itself.  (Joining in
 // the own-keys kernel, behind its pages, was slower: its few rows per CTA
 // expose the latency of every plane's load.  512 rows x 16384 keys x 32 heads
-// of 128, with the prefix kernel of that time: 280 us against 230; now 180.)
+// of 128, with an earlier prefix kernel: 280 us against 230.)
+//
+// Figures in this file are GPU time per call, replayed from a CUDA graph in
+// runs of a few ms at 1965 MHz; those in pairs compare builds that differ in
+// what is described alone.  The present code: 512 rows x 16384 keys x 32/8
+// heads of 128 in BF16 176 us (202 in long runs, which the power limit holds
+// near 1640 MHz), 64 x 4001 x 28/4 of 128 22.5, 33 x 6000 x 8/2 of 256 27.1.
 #include <cuda.h>
 
 #include <algorithm>
@@ -188,7 +194,7 @@ struct Unit {
 // numbers, pages, partials, output) is hidden by other units: small rings,
 // two or three CTAs per SM (us, against rings that fill an SM's shared memory
 // and one CTA: 64 sequences of one row 25 / 31, 33 to 96 rows each 26 / 33, 512
-// single rows behind 16384 shared keys 180 / 243, where they also find room
+// rows behind 16384 shared keys 180 / 243, where they also find room
 // beside the prefix kernel).
 template <typename E, int HD, bool SPLITK, bool OWN>
 __global__ void __maxnreg__((HD == 256 ? 255 : kOwnRegs))
@@ -582,8 +588,8 @@ struct Ptc {
   static constexpr int S_COL = 0, O_COL = NT * 128;  // tile t: S at 128 t and 128 t + 64, O at O_COL + HD t
   // Registers per thread and the ring's depth leave the own-keys kernel's CTAs
   // (a warp per SM quarter, kOwnRegs) room on the SM: one beside two tiles, two
-  // beside one tile (64 rows, 4001 shared keys x 28/4 heads of 128: 21.4 us a
-  // call, against 25 with six stages and one).  head_dim 256 has none anyway.
+  // beside one tile (64 rows, 4001 shared keys x 28/4 heads of 128: 21.4 us,
+  // against 25 with six stages and one).  head_dim 256 has none anyway.
   static constexpr int REGS = 112;
   static constexpr int BESIDE = HD == 256 ? 0 : NT == 2 ? 1 : 2;
   static_assert(O_COL + NT * HD <= COLS, "TMEM columns");
@@ -1029,7 +1035,7 @@ Shape shape_of(const laya_kv_pages& c, const laya_prefix_args& a, int sms) {
   // 16-row tiles on mma.sync read the prefix once per tile, but start and end
   // sooner than the tensor-core kernel, which takes over at about ten tile-pages
   // of head_dim 64 per SM.  The square of head_dim counts: a tile's work per page
-  // and how few CTAs an SM holds (a call's us, mma.sync / tcgen05, tile-pages per
+  // and how few CTAs an SM holds (us, mma.sync / tcgen05, tile-pages per
   // SM: 32 x 1000 keys x 32/8 heads of 64 11.1 / 12.2 at 7, 16 x 4000 14.7 / 13.7
   // at 14; 4 x 2000 x 28/4 of 128 10.6 / 11.1 at 1.7, 16 x 1000 12.8 / 11.1 at 3;
   // 16 x 1500 x 8/2 of 256 16.2 / 12.0 at 1.3).

@@ -4,7 +4,7 @@
 // A call of these operators is a few microseconds of GPU work, and building
 // the outputs and reading eight tensors' sizes, strides and types through
 // Python attributes and ctypes took two to four times as long (16-20 us a
-// call, against 7-9 here), so this is the one part of the package that binds
+// call, against 4-11 here), so this is the one part of the package that binds
 // in C++.  It checks what a tensor says of itself; the sizes' sense is checked
 // by the entry points.  The functions here are called by laya_goish_b200.device.
 #include <ATen/ATen.h>

@@ -63,7 +63,9 @@ def check_status(device: int = 0) -> None:
 
 
 class PagePlan(NamedTuple):
-    """What page_plan computes, on the device (capacity c, n sequences)."""
+    """What page_plan computes, on the device (capacity c, n sequences).  One
+    allocation holds them all: who keeps one past the step (lens, say) keeps 24
+    bytes per row of the capacity, or clones it."""
 
     slots: torch.Tensor      # [c] int64: page * 64 + row, -1 without one
     positions: torch.Tensor  # [c] int32
@@ -151,7 +153,8 @@ def prefix_attention(q, pages: KVPages, prefix_pages, prefix_len: int, tables, l
 
 
 class TokenLogprobs(NamedTuple):
-    """What token_logprobs computes ([n] rows, c tokens, k alternatives)."""
+    """What token_logprobs computes ([n] rows, c tokens, k alternatives), in one
+    allocation."""
 
     logprobs: torch.Tensor      # [n, c] F32; 0 for token -1
     entropy: torch.Tensor       # [n] F32, nats
